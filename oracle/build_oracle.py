@@ -96,7 +96,7 @@ def build_reference(reference: str = DEFAULT_REFERENCE, force: bool = False, job
                     gpu: bool = True) -> list[str]:
     """Compile the reference sources in place into oracle/_ref/.  Returns the
     list of libraries built (empty when the reference checkout is absent)."""
-    if not os.path.isdir(reference):
+    if not os.path.isdir(reference) or not os.listdir(reference):  # absent, or an empty mount point
         return []
     os.makedirs(REF_OUT, exist_ok=True)
     todo = list(CPU_SHIMS) + (list(GPU_SHIMS) if gpu else [])
