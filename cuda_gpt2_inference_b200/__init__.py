@@ -38,7 +38,9 @@ KV_FLOATX, KV_8BIT = 0, 1
 OPT_USE_GRAPH, OPT_USE_PDL, OPT_SPLITS, OPT_STEPS_PER_GRAPH, OPT_PERSISTENT, OPT_POLL_LIMIT, OPT_PREFILL = \
     1, 2, 3, 4, 5, 6, 7
 # device error codes (gpt2b_device_error)
+DEVERR_BAD_POS = 3
 DEVERR_GRID_TIMEOUT = 5
+DEVERR_BAD_BLOCK = 6
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -103,6 +105,13 @@ _SIGS = {
     "gpt2b_matmul_forward_w8_fp8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
     "gpt2b_matmul_forward_w8_i8_f32out": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "gpt2b_matmul_forward_w8_fp8_f32out": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "gpt2b_kv_block_tables": (_I, [_P] * 12 + [_I] * 5 + [_P]),
+    "gpt2b_kv_cache_write_w4": (_I, [_P] * 4 + [_I] * 7 + [_P]),
+    "gpt2b_kv_cache_read_w4": (_I, [_P] * 4 + [_I] * 5 + [_P]),
+    "gpt2b_attention_paged_w4_workspace": (_I, [_I] * 4 + [_P]),
+    "gpt2b_attention_forward_paged_w4": (_I, [_P] * 7 + [_I] * 10 + [_F, _P, _SZ, _P]),
+    "gpt2b_softmax_probs": (_I, [_P, _P, _I, _I, _I, _I, _F, _P]),
+    "gpt2b_verify_draft_tokens": (_I, [_P] * 8 + [_I] * 6 + [_P]),
     "gpt2b_read_header": (_I, [_S, _P, _P]),
     "gpt2b_engine_create_from_file": (_I, [_S, _S, _I, _I, _P]),
     "gpt2b_engine_create_from_buffer": (_I, [_P, _SZ, _P, _SZ, _I, _I, _P]),

@@ -174,6 +174,9 @@ int attention_device_error();
 int norm_device_error();
 int sampler_device_error();
 int persistent_device_error();
+int paged_kv_device_error();
+int paged_attention_device_error();
+int verify_device_error();
 
 // Chooses rows per tile / stages / grid for an M x K matrix of kind wk.
 // Returns false when the shape cannot be tiled (row larger than a tile).

@@ -1,0 +1,294 @@
+// paged_kv.cu -- a paged KV cache held in 4 bits: block tables and slot maps
+// from request lengths, append and read-back.
+//
+// Cache of one layer: codes u8 [num_blocks][K|V][NKV][block_size][hs/2] (byte i
+// of a row: channel 2i in the low nibble, 2i+1 in the high one) and steps
+// [num_blocks][K|V][NKV][block_size][hs/64][2] BF16 (step s, low end lo of each
+// group of 64 channels).  value = code * s + lo.  4.5 bits a value.
+#include "common.cuh"
+#include "internal.h"
+#include "paged_kv.cuh"
+
+#include <limits.h>
+
+namespace gpt2b {
+
+GPT2B_DEFINE_ERROR_READER(paged_kv_device_error)
+
+// ---------------------------------------------------------------------------
+// block tables and slot maps
+// ---------------------------------------------------------------------------
+// Every CTA computes the two exclusive prefix sums over the requests (rows, and
+// blocks to be taken from the free list) for itself and then writes its share of
+// the rows and of the table entries, so one launch does without a grid barrier:
+// 12 bytes a request from L2 against a second launch.  Nothing that a CTA reads
+// is written by another: a row's block is either one that the request held
+// (below have, which no CTA writes) or comes from the free list directly.
+constexpr int kTabThreads = 256;
+
+struct TableArgs {
+    int* block_table;
+    long long* slot_map;
+    int *positions, *row_start, *seq_lens, *blocks_out, *free_left;
+    const int *ctx_lens, *new_lens, *blocks_have, *free_list, *free_count;
+    int B, max_blocks, block_size, max_rows, free_cap;
+};
+
+struct Request {
+    long long end;  // context + new rows
+    int n, ctx, have;
+};
+__device__ __forceinline__ Request load_request(const TableArgs& a, int b) {
+    Request r;
+    r.ctx = max(a.ctx_lens[b], 0);
+    r.n = max(a.new_lens[b], 0);
+    r.have = min(max(a.blocks_have[b], 0), a.max_blocks);
+    r.end = (long long)r.ctx + r.n;
+    return r;
+}
+
+__global__ void __launch_bounds__(kTabThreads) block_tables_kernel(TableArgs a) {
+    extern __shared__ int tab_smem[];
+    int* row_end = tab_smem;        // [B] inclusive prefix of rows, at most max_rows
+    int* excl = tab_smem + a.B;     // [B] exclusive prefix of blocks asked for, at most INT_MAX
+    int* need = tab_smem + 2 * a.B; // [B] blocks asked for, or -1 where the request is not served
+    __shared__ long long w_rows[kTabThreads / 32], w_need[kTabThreads / 32];
+    __shared__ int s_take;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int F = min(max(*a.free_count, 0), a.free_cap);
+    const long long most = (long long)a.max_blocks * a.block_size;
+    if (tid == 0) s_take = 0;
+    long long rows0 = 0, need0 = 0;  // totals of the requests before this pass
+    for (int base = 0; base < a.B; base += kTabThreads) {
+        const int b = base + tid;
+        Request r{};
+        if (b < a.B) r = load_request(a, b);
+        // a refused request asks for no block; whether its rows fit is known after the first scan
+        long long rows = r.n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, rows, o);
+            if (lane >= o) rows += v;
+        }
+        if (lane == 31) w_rows[w] = rows;
+        __syncthreads();
+        long long before = rows0, all_rows = 0;
+        for (int k = 0; k < kTabThreads / 32; k++) {
+            if (k < w) before += w_rows[k];
+            all_rows += w_rows[k];
+        }
+        rows += before;
+        const bool fits = b < a.B && r.end <= most && rows <= a.max_rows;
+        const long long blocks = (r.end + a.block_size - 1) / a.block_size;
+        const int nd = fits && blocks > r.have ? (int)(blocks - r.have) : 0;
+        long long upto = nd;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) w_need[w] = upto;
+        __syncthreads();
+        long long nbefore = need0, all_need = 0;
+        for (int k = 0; k < kTabThreads / 32; k++) {
+            if (k < w) nbefore += w_need[k];
+            all_need += w_need[k];
+        }
+        upto += nbefore;
+        if (b < a.B) {
+            const bool served = fits && (nd == 0 || upto <= F);
+            row_end[b] = (int)min(rows, (long long)a.max_rows);
+            excl[b] = (int)min(upto - nd, (long long)INT_MAX);
+            need[b] = served ? nd : -1;
+            if (served && nd) atomicMax(&s_take, (int)upto);
+            if (blockIdx.x == 0) {
+                a.row_start[b + 1] = row_end[b];
+                a.seq_lens[b] = served ? (int)r.end : 0;
+                a.blocks_out[b] = r.have + (served ? nd : 0);
+            }
+        }
+        rows0 += all_rows;
+        need0 += all_need;
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        a.row_start[0] = 0;
+        *a.free_left = F - s_take;
+    }
+    // table entries of the new blocks: a warp per request
+    for (int b = blockIdx.x * (kTabThreads / 32) + w; b < a.B; b += gridDim.x * (kTabThreads / 32)) {
+        const int nd = need[b];
+        if (nd <= 0) continue;
+        const int have = min(max(a.blocks_have[b], 0), a.max_blocks);
+        for (int j = lane; j < nd; j += 32)
+            a.block_table[(size_t)b * a.max_blocks + have + j] = a.free_list[F - 1 - excl[b] - j];
+    }
+    // rows
+    for (long long i = (long long)blockIdx.x * kTabThreads + tid; i < a.max_rows; i += (long long)gridDim.x * kTabThreads) {
+        const int r = (int)i;
+        int lo = 0, hi = a.B;  // first request whose rows end behind r
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (row_end[mid] > r) hi = mid; else lo = mid + 1;
+        }
+        long long slot = -1;
+        int pos = 0;
+        if (lo < a.B && need[lo] >= 0) {
+            const Request q = load_request(a, lo);
+            // a served request's rows are not cut, so it begins n rows before its end
+            pos = q.ctx + (r - (row_end[lo] - q.n));
+            const int j = pos / a.block_size;
+            const int blk = j < q.have ? a.block_table[(size_t)lo * a.max_blocks + j]
+                                       : a.free_list[F - 1 - excl[lo] - (j - q.have)];
+            slot = blk < 0 ? -1 : (long long)blk * a.block_size + pos % a.block_size;
+        }
+        a.slot_map[r] = slot;
+        a.positions[r] = pos;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// append and read-back
+// ---------------------------------------------------------------------------
+// 8 threads hold a group of 64 channels, 8 channels each (one 16-byte load, one
+// 4-byte store of codes); the group's ends come from three shuffles.  All sums
+// are of two terms; explicit rn operations keep the codes independent of
+// contraction and of the fast-math division.
+__global__ void __launch_bounds__(256)
+    kv_write_w4_kernel(uint8_t* codes, uint32_t* scales, const __nv_bfloat16* qkv, const long long* slot_map, int rows,
+                       int NH, int NKV, int hs, int ld, long long slots, int block_size) {
+    const int per_row = 2 * NKV * hs / 8;
+    const long long total = (long long)rows * per_row, step = (long long)gridDim.x * blockDim.x;
+    const int NG = hs / kW4Group;
+    // per_row is a multiple of 8, so the 8 threads of a group are active together
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int row = (int)(i / per_row), c = (int)(i % per_row) * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(qkv + (size_t)row * ld + (size_t)NH * hs + c);
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) { x[2 * k] = bf16lo(u[k]); x[2 * k + 1] = bf16hi(u[k]); }
+        float lo = x[0], hi = x[0];
+        bool fin = true;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            lo = fminf(lo, x[k]);
+            hi = fmaxf(hi, x[k]);
+            fin = fin && (__float_as_uint(x[k]) & 0x7f800000u) != 0x7f800000u;
+        }
+        const unsigned group = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(group, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(group, hi, o));
+        }
+        fin = __ballot_sync(group, fin) == group;
+        uint32_t meta;
+        uint32_t word = w4_encode8(x, lo, hi, fin, meta);
+        const long long slot = slot_map[row];
+        if (slot < 0) continue;
+        if (slot >= slots) { report_device_error(GPT2B_DEVERR_BAD_BLOCK); continue; }
+        const int kv = c / (NKV * hs), h = (c / hs) % NKV, d = c % hs;
+        const size_t blk = (size_t)(slot / block_size), off = (size_t)(slot % block_size);
+        const size_t line = ((blk * 2 + kv) * NKV + h) * block_size + off;
+        *reinterpret_cast<uint32_t*>(codes + line * (hs / 2) + d / 2) = word;
+        if ((d & (kW4Group - 1)) == 0) scales[line * NG + d / kW4Group] = meta;
+    }
+}
+
+__global__ void __launch_bounds__(256)
+    kv_read_w4_kernel(__nv_bfloat16* out, const uint8_t* codes, const uint32_t* scales, const long long* slot_map, int rows,
+                      int NKV, int hs, long long slots, int block_size) {
+    const int per_row = 2 * NKV * hs / 8;
+    const long long total = (long long)rows * per_row, step = (long long)gridDim.x * blockDim.x;
+    const int NG = hs / kW4Group;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int row = (int)(i / per_row), c = (int)(i % per_row) * 8;
+        const long long slot = slot_map[row];
+        uint32_t r[4] = {0u, 0u, 0u, 0u};
+        if (slot >= slots) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
+        if (slot >= 0 && slot < slots) {
+            const int kv = c / (NKV * hs), h = (c / hs) % NKV, d = c % hs;
+            const size_t blk = (size_t)(slot / block_size), off = (size_t)(slot % block_size);
+            const size_t line = ((blk * 2 + kv) * NKV + h) * block_size + off;
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + line * (hs / 2) + d / 2);
+            const uint32_t meta = scales[line * NG + d / kW4Group];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(w4_value(word, meta, 2 * k), w4_value(word, meta, 2 * k + 1));
+                r[k] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+        }
+        *reinterpret_cast<uint4*>(out + (size_t)row * per_row * 8 + c) = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+}
+
+// a grid of at most 8 CTAs an SM for `work` threads of 256-thread CTAs
+static int stride_grid(long long work) {
+    const long long g = (work + 255) / 256, most = (long long)sm_count() * 8;
+    return (int)(g < 1 ? 1 : (g < most ? g : most));
+}
+
+}  // namespace gpt2b
+
+using namespace gpt2b;
+
+extern "C" {
+
+int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions, int* row_start, int* seq_lens,
+                          int* blocks_out, int* free_left, const int* ctx_lens, const int* new_lens,
+                          const int* blocks_have, const int* free_list, const int* free_count, int B, int max_blocks,
+                          int block_size, int max_rows, int free_cap, gpt2b_stream_t stream) {
+    if (B <= 0 || max_blocks <= 0 || block_size <= 0 || max_rows < 0 || free_cap < 0) return GPT2B_ERR_INVALID_ARG;
+    if (!block_table || !row_start || !seq_lens || !blocks_out || !free_left || !ctx_lens || !new_lens || !blocks_have ||
+        !free_count)
+        return GPT2B_ERR_INVALID_ARG;
+    if ((max_rows > 0 && (!slot_map || !positions)) || (free_cap > 0 && !free_list)) return GPT2B_ERR_INVALID_ARG;
+    // every CTA reads these while one writes the new ones
+    if (blocks_out == blocks_have || free_left == free_count || seq_lens == ctx_lens || seq_lens == new_lens)
+        return GPT2B_ERR_INVALID_ARG;
+    if (B > kTableMaxRequests || (long long)max_blocks * block_size > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
+    TableArgs a{block_table, slot_map, positions, row_start, seq_lens, blocks_out, free_left, ctx_lens, new_lens,
+                blocks_have, free_list, free_count, B, max_blocks, block_size, max_rows, free_cap};
+    static unsigned long long mask = 0;  // 4096 requests take 48 KB
+    if (const cudaError_t e = ensure_smem_limit(block_tables_kernel, &mask)) return status_from(e);
+    long long grid = ((long long)max_rows + kTabThreads * 4 - 1) / (kTabThreads * 4);
+    if (grid < 1) grid = 1;
+    if (grid > sm_count()) grid = sm_count();
+    return status_from(launch_k(block_tables_kernel, dim3((unsigned)grid), dim3(kTabThreads), 3 * sizeof(int) * (size_t)B,
+                                (cudaStream_t)stream, false, a));
+}
+
+static int w4_check(const void* codes, const void* scales, int NKV, int hs, int num_blocks, int block_size) {
+    if (NKV <= 0 || num_blocks <= 0 || block_size <= 0 || !codes || !scales) return GPT2B_ERR_INVALID_ARG;
+    if ((hs != 64 && hs != 128) || block_size % kW4Tile != 0) return GPT2B_ERR_UNSUPPORTED;
+    if (!aligned16(codes) || !aligned16(scales)) return GPT2B_ERR_ALIGNMENT;
+    return GPT2B_OK;
+}
+
+int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_t* qkv, const long long* slot_map, int rows,
+                            int NH, int NKV, int hs, int ld, int num_blocks, int block_size, gpt2b_stream_t stream) {
+    int rc = w4_check(kv_cache, kv_scale, NKV, hs, num_blocks, block_size);
+    if (rc) return rc;
+    if (rows < 0 || NH <= 0 || (rows > 0 && (!qkv || !slot_map))) return GPT2B_ERR_INVALID_ARG;
+    if (((long long)NH + 2ll * NKV) * hs > ld) return GPT2B_ERR_INVALID_ARG;
+    if (!aligned16(qkv) || ld % 8 != 0) return GPT2B_ERR_ALIGNMENT;
+    if (rows == 0) return GPT2B_OK;
+    return status_from(launch_k(kv_write_w4_kernel, dim3(stride_grid((long long)rows * (2 * NKV * hs / 8))), dim3(256), 0,
+                                (cudaStream_t)stream, false, kv_cache, (uint32_t*)kv_scale, (const __nv_bfloat16*)qkv, slot_map,
+                                rows, NH, NKV, hs, ld, (long long)num_blocks * block_size, block_size));
+}
+
+int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_t* kv_scale, const long long* slot_map,
+                           int rows, int NKV, int hs, int num_blocks, int block_size, gpt2b_stream_t stream) {
+    int rc = w4_check(kv_cache, kv_scale, NKV, hs, num_blocks, block_size);
+    if (rc) return rc;
+    if (rows < 0 || (rows > 0 && (!out || !slot_map))) return GPT2B_ERR_INVALID_ARG;
+    if (!aligned16(out)) return GPT2B_ERR_ALIGNMENT;
+    if (rows == 0) return GPT2B_OK;
+    return status_from(launch_k(kv_read_w4_kernel, dim3(stride_grid((long long)rows * (2 * NKV * hs / 8))), dim3(256), 0,
+                                (cudaStream_t)stream, false, (__nv_bfloat16*)out, kv_cache, (const uint32_t*)kv_scale, slot_map,
+                                rows, NKV, hs, (long long)num_blocks * block_size, block_size));
+}
+
+}  // extern "C"

@@ -51,7 +51,8 @@ enum {
     GPT2B_DEVERR_BAD_TOKEN = 2,    /* token id outside [0, vocab) */
     GPT2B_DEVERR_BAD_POS = 3,      /* position outside [0, maxT) */
     GPT2B_DEVERR_PEER_TIMEOUT = 4, /* a cross-GPU flag wait hit its bound */
-    GPT2B_DEVERR_GRID_TIMEOUT = 5  /* a wait on another CTA of the persistent decode kernel hit its bound */
+    GPT2B_DEVERR_GRID_TIMEOUT = 5, /* a wait on another CTA of the persistent decode kernel hit its bound */
+    GPT2B_DEVERR_BAD_BLOCK = 6     /* a block or slot outside the paged cache; it was neither read nor written */
 };
 
 const char* gpt2b_status_string(int status);
@@ -220,6 +221,79 @@ int gpt2b_attention_forward_kv_large_bf16_noalloc(uint16_t* out, const uint16_t*
                                                   gpt2b_stream_t stream);
 
 /* ======================================================================== */
+/* Batches of requests over a paged 4-bit KV cache                           */
+/* ======================================================================== */
+/* No counterpart in the reference (one request, one contiguous cache).
+ *
+ * Rows.  The step's token rows of all requests are packed: request b has the
+ * rows [row_start[b], row_start[b+1]), its tokens in order (for a decoding
+ * request the last token, then its drafts).  Buffers may hold more rows than
+ * row_start[B]; the rows behind it are left as they were.
+ * Cache of one layer.  num_blocks blocks of block_size positions (a multiple of
+ * 16); NKV key/value heads (a divisor of the NH query heads) of hs = 64 or 128.
+ *   kv_cache u8   [num_blocks][2 (K|V)][NKV][block_size][hs/2]: 4-bit codes,
+ *                 byte i holds channel 2i (low nibble) and 2i+1 (high nibble);
+ *   kv_scale BF16 [num_blocks][2][NKV][block_size][hs/64][2]: per group of 64
+ *                 channels the step s and the low end lo.
+ * A channel's value is code * s + lo.  Slot = block * block_size + offset.
+ * Block tables are int32 [B][max_blocks]; entries behind a request's last block
+ * are not read.  kv_cache, kv_scale, qkv and out are 16-byte aligned.
+ * qkv rows are [Q (NH*hs) | K (NKV*hs) | V (NKV*hs)], ld elements apart. */
+
+/* Block tables and row maps of one step, from the requests' lengths.  Request b
+ * has ctx_lens[b] cached positions, new_lens[b] new rows (either may be 0;
+ * a negative one counts as 0) and blocks_have[b] blocks in its table row (more
+ * than its context needs where refused drafts were cut).  It needs
+ * max(0, ceil((ctx+new)/block_size) - have) more, which are taken from the end of
+ * free_list[0 .. *free_count) in request order and written to its table row.
+ * A request whose blocks do not fit max_blocks or whose rows do not fit max_rows
+ * is refused and asks for none; one whose blocks the free list cannot give
+ * counts as asking (nothing behind it is served first, unless it needs none) but
+ * takes none.  Writes
+ *   row_start [B+1]   prefix of new_lens (at most max_rows)
+ *   seq_lens [B]      ctx + new, 0 for a request that is not served
+ *   blocks_out [B]    blocks held afterwards
+ *   free_left [1]     free_list[0 .. *free_left) are still free
+ *   slot_map, positions [max_rows]  of each row; -1 and 0 for the rows of a request
+ *                     that is not served and behind the last request
+ * and changes nothing else, so the same call again gives the same result; the
+ * caller takes blocks_out and *free_left over as the next step's blocks_have and
+ * *free_count.  These must be different buffers from the inputs
+ * (GPT2B_ERR_INVALID_ARG).  free_cap is the length of free_list.  B <= 4096. */
+int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions, int* row_start, int* seq_lens,
+                          int* blocks_out, int* free_left, const int* ctx_lens, const int* new_lens,
+                          const int* blocks_have, const int* free_list, const int* free_count, int B, int max_blocks,
+                          int block_size, int max_rows, int free_cap, gpt2b_stream_t stream);
+/* Appends rows' K and V at slot_map[row]: per group of 64 channels s =
+ * bf16(max/15 - min/15) (0 below 2^-120), lo = min, code = round((x - lo)/s), ties
+ * to even, at most 15.  A group with a NaN or an infinity is held as NaN.  A
+ * negative slot skips the row; a slot outside the cache is skipped and reported
+ * (GPT2B_DEVERR_BAD_BLOCK).  The non-negative slots of a call must differ: of two
+ * rows with one slot, either may be held, or a mix of their groups. */
+int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_t* qkv, const long long* slot_map, int rows,
+                            int NH, int NKV, int hs, int ld, int num_blocks, int block_size, gpt2b_stream_t stream);
+/* Reads rows back as BF16 values: out [rows][2 (K|V)][NKV][hs]; zeros for a
+ * negative slot, and for one outside the cache, which is also reported. */
+int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_t* kv_scale, const long long* slot_map,
+                           int rows, int NKV, int hs, int num_blocks, int block_size, gpt2b_stream_t stream);
+/* Attention of the packed rows over the cache: row i of request b's n rows sees
+ * the positions [0, seq_lens[b] - n + i] (its own K and V appended before), so
+ * drafts are causal among themselves.  out row: [NH*hs] BF16, zeros where a row
+ * sees nothing.  seq_lens beyond max_blocks * block_size and row_start outside
+ * [0, rows] are cut and reported (GPT2B_DEVERR_BAD_POS); a block outside the cache
+ * is left out and reported (GPT2B_DEVERR_BAD_BLOCK).  scale: of the scores
+ * (1/sqrt(hs)).  max_q: the most rows a request has, a hint for the tile choice.
+ * workspace: gpt2b_attention_paged_w4_workspace() bytes for the same NH, NKV, hs,
+ * max_q on the current device, 16-byte aligned; needs no initialisation and holds
+ * nothing between calls; calls that can overlap need one each.  B <= 4096. */
+int gpt2b_attention_paged_w4_workspace(int NH, int NKV, int hs, int max_q, size_t* bytes);
+int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const uint8_t* kv_cache, const uint16_t* kv_scale,
+                                     const int* block_table, const int* seq_lens, const int* row_start, int B, int rows,
+                                     int NH, int NKV, int hs, int ld, int num_blocks, int block_size, int max_blocks,
+                                     int max_q, float scale, void* workspace, size_t workspace_bytes,
+                                     gpt2b_stream_t stream);
+
+/* ======================================================================== */
 /* LayerNorm, residual, embedding                                            */
 /* ======================================================================== */
 /* out = (x-mean)*rstd*w + b per row of C; mean/rstd (float, may be NULL).
@@ -261,6 +335,34 @@ int gpt2b_gpu_argmax(int* d_token, const float* logits, int B, int V, int ld, gp
  * reference's ppl_record_nll computes on the host after copying the logits
  * back (Inference_gpt2/dump_utils.h:63-79), here on the device. */
 int gpt2b_logits_nll(float* d_nll, const float* logits, int V, const int* d_token, gpt2b_stream_t stream);
+
+/* probs[r] = softmax(logits[r] / temperature) over the first V logits of each
+ * row (rows ld_* apart), FP32.  temperature is 0 or at least 1e-30; 0: 1 at the largest logit (lowest
+ * index on ties), 0 elsewhere.  A row with nothing above -infinity gives zeros; a
+ * NaN or +infinity gives NaN (temperature 0 passes over NaN).  probs may be
+ * logits.  No counterpart in the reference (its sampler keeps no probabilities). */
+int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int ld_logits, int ld_probs, float temperature,
+                        gpt2b_stream_t stream);
+/* Verification of drafted tokens by rejection sampling.  Rows are packed as for
+ * the paged cache: request b has the rows [r0, r1) = [row_start[b], row_start[b+1]),
+ * tokens[r0] its last token, tokens[r0+1 .. r1) its drafts; target_probs[r] is the
+ * target's distribution of the token behind row r, draft_probs[r] the one that draft
+ * tokens[r+1] was drawn from (NULL: drafts were certain, probability 1).
+ * Draft x = tokens[r+1] is accepted while u_accept[r] * draft_probs[r][x] <
+ * target_probs[r][x].  At the first refusal one token is drawn from
+ * max(target - draft, 0) (draft_probs NULL: target with x left out; where that
+ * leaves nothing: target); with all accepted, from the last row's target_probs.
+ * The drawn token is the first k whose cumulative weight exceeds u_sample[b] *
+ * total, else the last k of positive weight, or -1 where a row has no positive
+ * weight.  Products, weights and sums are in 64 bits.  A draft outside [0, V) ends
+ * the drafts: the token is drawn from that row's target_probs, as if it were last.
+ * out_tokens [B][max_out]: the accepted drafts, the drawn token, then -1; at most
+ * max_out - 1 drafts are looked at.  n_accepted [B].  A request without rows gets
+ * -1s and 0.  row_start outside [0, rows] is cut and reported
+ * (GPT2B_DEVERR_BAD_POS).  No counterpart in the reference. */
+int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* tokens, const float* target_probs,
+                              const float* draft_probs, const int* row_start, const float* u_accept, const float* u_sample,
+                              int B, int rows, int V, int ld_target, int ld_draft, int max_out, gpt2b_stream_t stream);
 
 /* ======================================================================== */
 /* Prompt GEMM on the tensor cores (tcgen05)                                */
