@@ -1,7 +1,25 @@
 // paged_attention.cu -- attention over the paged 4-bit KV cache.
 //
 // A row i of a request's n rows sees the positions [0, len - n + i]; query head h
-// reads key/value head h / (NH/NKV).  Softmax statistics in FP32 (online).
+// reads key/value head h / (NH/NKV).  The (row, head) pairs that share a key/value
+// head are the columns of one tile, so its codes are read and decoded once for all
+// of them:
+//   S[pos][col] = s_pos (codes_K[pos] . q[col]) + lo_pos sum(q[col])
+//   out[ch][col] = sum_pos codes_V[pos][ch] (P[pos][col] s_pos) + sum_pos P lo_pos
+// Step and low end are factors of a whole position, so the products take the codes
+// themselves (0..15) as FP16 operands of mma.sync m16n8k16, positions (K) or
+// channels (V) in its 16 rows, 8 columns in its N.
+//
+// Codes as FP16.  A nibble masked in place in bits 0..3 or 4..7 of a 16-bit half is
+// the FP16 subnormal code * 2^-24 or code * 2^-20: one AND a pair, no conversion and
+// no offset to take off again (0.6 instructions a code).  The tensor cores multiply
+// subnormals exactly; the powers of two are put right in q (K: even nibbles carry a
+// factor of 16) and in the final scaling (V).
+//
+// Why mma.sync and not tcgen05: an operand of tcgen05.mma has 64 rows or more and
+// lies in shared or tensor memory, so every decoded code would be written and read
+// there again; here a tile has 1..16 columns, and the codes go from a register to
+// the tensor core that multiplies them.
 #include "paged_kv.cuh"
 #include "internal.h"
 
@@ -19,76 +37,658 @@ struct PagedAttnArgs {
     const uint32_t* scales;
     const int *block_table, *seq_lens, *row_start;
     int B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks;
-    float scale;
+    float scale_log2;  // softmax scale * log2(e)
+    float* ws;
 };
 
-constexpr int kPaThreads = 128;
+constexpr int kPaWarps = 4;
+constexpr int kPaThreads = 32 * kPaWarps;
+constexpr int kPaStep = 32;                     // positions a warp takes at a time
+constexpr int kPaUnit = kPaStep * kPaWarps;     // positions of a unit of the work partition
+constexpr int kPaStages = 3;                    // steps in flight a warp
 
-// One CTA per (row, query head): its 4 warps take the positions in turn, a lane
-// holds hs/32 channels, and the warps' states are merged at the end.
-template <int HS>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(PagedAttnArgs a) {
-    constexpr int CH = HS / 32, NG = HS / kW4Group;
-    const int row = blockIdx.x / a.NH, head = blockIdx.x % a.NH, kvh = head / (a.NH / a.NKV);
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int lo = 0, hi = a.B;  // first request that ends behind the row
+template <int NG, int NT> struct PaShape {
+    static constexpr int kHS = NG * kW4Group, kCols = 8 * NT;
+    static constexpr int kCodeBytes = kPaStep * 32 * NG, kMetaBytes = kPaStep * 4 * NG;
+    static constexpr int kStageBytes = 2 * (kCodeBytes + kMetaBytes);
+    static constexpr int kRing = kPaWarps * kPaStages * kStageBytes;
+    static constexpr int kPitch = kHS + 1;  // floats between the columns of a warp's slab
+    static constexpr int kMerge = (kPaWarps * kCols * kPitch + 2 * kPaWarps * kCols) * 4;
+    static constexpr int kSmem = ((kRing > kMerge ? kRing : kMerge) + 15) & ~15;
+    static constexpr int kCtas = NG * NT <= 2 ? 4 : 3;  // resident CTAs an SM (registers)
+    static constexpr int kSlot = kCols * (kHS + 2);     // floats of a partial result
+};
+
+// ---------------------------------------------------------------------------
+// work partition
+// ---------------------------------------------------------------------------
+// A segment is a (request, key/value head, tile of columns); it has ceil(len/128)
+// units.  The units of all segments are numbered in one row and dealt out in equal
+// contiguous runs to the resident CTAs, whatever the lengths are: a long request is
+// split over many CTAs, short ones share one.  A CTA writes a finished segment to
+// `out`, and the piece of a segment that it shares with its neighbours to one of its
+// two slots (0: the segment began before its run, 1: it goes on behind it).
+struct PaRequest {
+    int r0, n, len, chunks, units;
+};
+__device__ __forceinline__ PaRequest pa_request(const PagedAttnArgs& a, int b, int cols, bool report) {
+    PaRequest r;
+    const int s0 = a.row_start[b], s1 = a.row_start[b + 1], l0 = a.seq_lens[b];
+    r.r0 = min(max(s0, 0), a.rows);
+    const int r1 = min(max(s1, r.r0), a.rows);
+    r.n = r1 - r.r0;
+    r.len = min(max(l0, 0), a.max_blocks * a.block_size);
+    if (report && (r.r0 != s0 || r1 != s1 || l0 > r.len)) report_device_error(GPT2B_DEVERR_BAD_POS);
+    r.chunks = (r.n * (a.NH / a.NKV) + cols - 1) / cols;
+    r.units = max(1, (r.len + kPaUnit - 1) / kPaUnit);  // a request that sees nothing still gets its zeros
+    return r;
+}
+
+// pre[b] = units of the requests before b, pre[B] = all; every thread of the CTA calls it.
+__device__ __forceinline__ void pa_scan(const PagedAttnArgs& a, int cols, long long* pre, long long* wsum, bool report) {
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    long long base = 0;
+    if (tid == 0) pre[0] = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kPaThreads) {
+        const int b = b0 + tid;
+        long long v = 0;
+        if (b < a.B) {
+            const PaRequest r = pa_request(a, b, cols, report);
+            v = (long long)a.NKV * r.chunks * r.units;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) wsum[w] = v;
+        __syncthreads();
+        long long all = 0;
+#pragma unroll
+        for (int k = 0; k < kPaWarps; k++) {
+            if (k < w) v += wsum[k];
+            all += wsum[k];
+        }
+        if (b < a.B) pre[b + 1] = base + v;
+        base += all;
+        __syncthreads();
+    }
+}
+// the request that holds unit u
+__device__ __forceinline__ int pa_find(const long long* pre, int B, long long u) {
+    int lo = 0, hi = B - 1;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (a.row_start[mid + 1] > row) hi = mid; else lo = mid + 1;
+        if (pre[mid + 1] > u) hi = mid; else lo = mid + 1;
     }
-    if (lo >= a.B || a.row_start[lo] > row) return;
-    int len = max(a.seq_lens[lo], 0);
-    if (len > a.max_blocks * a.block_size) {
-        len = a.max_blocks * a.block_size;
-        report_device_error(GPT2B_DEVERR_BAD_POS);
-    }
-    if (a.row_start[lo + 1] > a.rows) report_device_error(GPT2B_DEVERR_BAD_POS);
-    const int n = min(a.row_start[lo + 1], a.rows) - a.row_start[lo];
-    const int seen = len - n + (row - a.row_start[lo]) + 1;
-    float q[CH], o[CH], m = -FLT_MAX, l = 0.0f;
+    return lo;
+}
+
+// ---------------------------------------------------------------------------
+// PTX
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t mov_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float meta_step(uint32_t m) { return __uint_as_float(m << 16); }
+__device__ __forceinline__ float meta_low(uint32_t m) { return __uint_as_float(m & 0xffff0000u); }
+__device__ __forceinline__ float pow2_field(int field) { return __uint_as_float((uint32_t)field << 23); }
+
+constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // nibbles as code * 2^-24 / code * 2^-20
+
+// Tile row r of 8 holds the position r ^ (r >> 2): then the 8 rows of a K load (8 bytes a lane) and
+// the 4 even or odd rows of a V load (4 bytes a lane) each fall in distinct banks.
+__device__ __forceinline__ int tile_pos(int r) { return r ^ ((r >> 2) & 1); }
+
+template <int NG, int NT>
+__global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn_kernel(PagedAttnArgs a) {
+    using Sh = PaShape<NG, NT>;
+    constexpr int HS = Sh::kHS, COLS = Sh::kCols;
+    extern __shared__ __align__(16) unsigned char smem[];
+    long long* pre = reinterpret_cast<long long*>(smem + Sh::kSmem);
+    __shared__ long long wsum[kPaWarps];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int ratio = a.NH / a.NKV;
+
+    pa_scan(a, COLS, pre, wsum, blockIdx.x == 0);
+    const long long total = pre[a.B];
+    const long long G = min((long long)gridDim.x, total);
+    if (blockIdx.x >= G) return;
+    long long u = total * blockIdx.x / G;
+    const long long u_end = total * (blockIdx.x + 1) / G;
+    int b = pa_find(pre, a.B, u);
+
+    // this lane's places in a stage
+    const uint32_t ring = smem_addr(smem) + w * (kPaStages * Sh::kStageBytes);
+    const uint32_t k_off = tile_pos(g) * 32 + 8 * t;           // K codes, rows g and (+ 256) g + 8
+    const uint32_t m_off = tile_pos(g) * 4 * NG;               // steps of the same rows
+    const uint32_t va_off = tile_pos(2 * t) * 32 + 4 * g;      // V codes of the row pairs (2t, 2t + 1)
+    const uint32_t vb_off = tile_pos(2 * t + 1) * 32 + 4 * g;
+
+    while (u < u_end) {
+        while (pre[b + 1] <= u) b++;
+        const PaRequest rq = pa_request(a, b, COLS, false);
+        const long long per_head = (long long)rq.chunks * rq.units, local = (u - pre[b]) % per_head;
+        const int kvh = (int)((u - pre[b]) / per_head);
+        const int chunk = (int)(local / rq.units), t0 = (int)(local % rq.units);
+        const int t1 = (int)min((long long)rq.units, t0 + (u_end - u));
+        u += t1 - t0;
+        const int ncol = min(COLS, rq.n * ratio - chunk * COLS);
+        const int last = rq.len - rq.n;  // row i sees positions <= last + i
+        const int row_lo = chunk * COLS / ratio, row_hi = (chunk * COLS + ncol - 1) / ratio;
+        const int seen_all = last + row_lo;                               // seen by every column
+        const int p_end = min(min(rq.len, last + row_hi + 1), t1 * kPaUnit);  // behind the last position seen
+
+        // ---- queries: column g of each tile as the B operand, scaled to [2^10, 2^11) at their largest
+        uint32_t q[NT][NG][4][2];
+        float cf[NT][2], qs[NT][NG][2];
+        int lim[NT][2];
 #pragma unroll
-    for (int k = 0; k < CH; k++) {
-        q[k] = to_f(a.qkv[(size_t)row * a.ld + head * HS + lane * CH + k]) * a.scale;
-        o[k] = 0.0f;
-    }
-    for (int p = w; p < seen; p += kPaThreads / 32) {
-        const int blk = a.block_table[(size_t)lo * a.max_blocks + p / a.block_size];
-        if (blk < 0 || blk >= a.num_blocks) {
-            report_device_error(GPT2B_DEVERR_BAD_BLOCK);
-            continue;
+        for (int nt = 0; nt < NT; nt++) {
+            const int col = nt * 8 + g;
+            uint32_t raw[NG][8];  // words 2t and 2t + 1: 16 channels
+            float mx = 0.0f;
+            const int gc = chunk * COLS + col;
+            const __nv_bfloat16* src = a.qkv + (size_t)(rq.r0 + gc / ratio) * a.ld + (size_t)(kvh * ratio + gc % ratio) * HS;
+#pragma unroll
+            for (int ng = 0; ng < NG; ng++) {
+                uint4 x = make_uint4(0, 0, 0, 0), y = x;
+                if (col < ncol) {
+                    x = *reinterpret_cast<const uint4*>(src + ng * kW4Group + 16 * t);
+                    y = *reinterpret_cast<const uint4*>(src + ng * kW4Group + 16 * t + 8);
+                }
+                raw[ng][0] = x.x; raw[ng][1] = x.y; raw[ng][2] = x.z; raw[ng][3] = x.w;
+                raw[ng][4] = y.x; raw[ng][5] = y.y; raw[ng][6] = y.z; raw[ng][7] = y.w;
+#pragma unroll
+                for (int k = 0; k < 8; k++) mx = fmaxf(mx, fmaxf(fabsf(bf16lo(raw[ng][k])), fabsf(bf16hi(raw[ng][k]))));
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const int field = min(264 - (int)(__float_as_uint(mx) >> 23), 254);
+            const float f = pow2_field(field);
+            const float c = a.scale_log2 * 1048576.0f * pow2_field(254 - field);  // D is in units of 2^-20 / f
+            cf[nt][0] = __shfl_sync(0xffffffffu, c, 8 * t);
+            cf[nt][1] = __shfl_sync(0xffffffffu, c, 8 * t + 4);
+#pragma unroll
+            for (int ng = 0; ng < NG; ng++) {
+                float v[16], s = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    v[2 * k] = bf16lo(raw[ng][k]) * f;
+                    v[2 * k + 1] = bf16hi(raw[ng][k]) * f;
+                    s += v[2 * k] + v[2 * k + 1];
+                }
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s *= 9.5367431640625e-7f;  // 2^-20
+                qs[nt][ng][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+                qs[nt][ng][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float* z = v + 8 * e + 2 * h;
+                        q[nt][ng][2 * e + h][0] = f16x2(z[0] * 16.0f, z[4] * 16.0f);
+                        q[nt][ng][2 * e + h][1] = f16x2(z[1], z[5]);
+                    }
+            }
+#pragma unroll
+            for (int c2 = 0; c2 < 2; c2++) {
+                const int cc = nt * 8 + 2 * t + c2;
+                lim[nt][c2] = cc < ncol ? last + (chunk * COLS + cc) / ratio : rq.len - 1;
+            }
         }
-        const size_t kl = (((size_t)blk * 2) * a.NKV + kvh) * a.block_size + p % a.block_size;
-        const size_t vl = kl + (size_t)a.NKV * a.block_size;
-        const int word = lane * CH / 8, sh = lane * CH % 8, g = lane * CH / kW4Group;
-        const uint32_t kw = reinterpret_cast<const uint32_t*>(a.codes + kl * (HS / 2))[word] >> (4 * sh);
-        const uint32_t vw = reinterpret_cast<const uint32_t*>(a.codes + vl * (HS / 2))[word] >> (4 * sh);
-        const uint32_t km = a.scales[kl * NG + g], vm = a.scales[vl * NG + g];
-        float s = 0.0f;
+
+        float m[NT][2], l[NT][2], az[NT][NG][2], acc[NT][NG][4][4];
 #pragma unroll
-        for (int k = 0; k < CH; k++) s += q[k] * w4_value(kw, km, k);
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), f = __expf(m - mn), e = __expf(s - mn);
-        m = mn;
-        l = l * f + e;
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < CH; k++) o[k] = o[k] * f + e * w4_value(vw, vm, k);
-    }
-    __shared__ float so[kPaThreads / 32][HS], sm[kPaThreads / 32], sl[kPaThreads / 32];
+            for (int ng = 0; ng < NG; ng++) {
+                az[nt][ng][0] = az[nt][ng][1] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < CH; k++) so[w][lane * CH + k] = o[k];
-    if (lane == 0) { sm[w] = m; sl[w] = l; }
-    __syncthreads();
-    float M = sm[0];
-    for (int k = 1; k < kPaThreads / 32; k++) M = fmaxf(M, sm[k]);
-    for (int d = threadIdx.x; d < HS; d += kPaThreads) {
-        float num = 0.0f, den = 0.0f;
-        for (int k = 0; k < kPaThreads / 32; k++) {
-            const float f = __expf(sm[k] - M);
-            num += f * so[k][d];
-            den += f * sl[k];
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[nt][ng][i][k] = 0.0f;
+            }
         }
-        a.out[(size_t)row * a.NH * HS + head * HS + d] = from_f<__nv_bfloat16>(den == 0.0f ? 0.0f : num / den);
+        int s_lim = -1, s_field = 127;  // V steps up to s_lim (BF16 bits) fit under the factor 2^(s_field - 127)
+
+        // ---- this warp's steps: positions first + it * kPaUnit
+        const int first = t0 * kPaUnit + w * kPaStep;
+        const int steps = first < p_end ? (p_end - first + kPaUnit - 1) / kPaUnit : 0;
+        const int* table = a.block_table + (size_t)b * a.max_blocks;
+        uint32_t bad = 0;  // two bits a stage: tiles whose block lies outside the cache
+        int blk[2];        // the blocks of the next step to be issued
+
+        auto fetch = [&](int it) {
+            const int p = first + it * kPaUnit;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (it < steps && p + 16 * j < p_end) blk[j] = table[(p + 16 * j) / a.block_size];
+        };
+        auto issue = [&](int it) {
+            if (it < steps) {
+                const int stage = it % kPaStages, p = first + it * kPaUnit;
+                const uint32_t base = ring + stage * Sh::kStageBytes;
+                bad &= ~(3u << (2 * stage));
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if (p + 16 * j >= p_end) continue;
+                    if (blk[j] < 0 || blk[j] >= a.num_blocks) {
+                        bad |= 1u << (2 * stage + j);
+                        if (lane == 0) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
+                        continue;
+                    }
+                    const size_t kl = (((size_t)blk[j] * 2) * a.NKV + kvh) * a.block_size + (p + 16 * j) % a.block_size;
+                    const size_t vl = kl + (size_t)a.NKV * a.block_size;
+                    const uint8_t* kc = a.codes + kl * (HS / 2);
+                    const uint8_t* vc = a.codes + vl * (HS / 2);
+#pragma unroll
+                    for (int k = 0; k < NG; k++) {
+                        const int i = lane + 32 * k, row = i / (2 * NG), c = i % (2 * NG);
+                        const uint32_t dst = base + (c >> 1) * (kPaStep * 32) + (16 * j + row) * 32 + (c & 1) * 16;
+                        cp_async16(dst, kc + i * 16);
+                        cp_async16(dst + Sh::kCodeBytes, vc + i * 16);
+                    }
+                    if (lane < 8 * NG) {
+                        const int i = lane % (4 * NG);
+                        const bool v = lane >= 4 * NG;
+                        cp_async16(base + 2 * Sh::kCodeBytes + (v ? Sh::kMetaBytes : 0) + 16 * j * 4 * NG + i * 16,
+                                   reinterpret_cast<const uint8_t*>(a.scales + (v ? vl : kl) * NG) + i * 16);
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+
+        fetch(0);
+#pragma unroll
+        for (int s = 0; s < kPaStages - 1; s++) {
+            issue(s);
+            fetch(s + 1);
+        }
+        for (int it = 0; it < steps; it++) {
+            __syncwarp();  // every lane has read the stage that is filled next
+            issue(it + kPaStages - 1);
+            fetch(it + kPaStages);
+            cp_async_wait<kPaStages - 1>();
+            __syncwarp();
+            const int stage = it % kPaStages, p0 = first + it * kPaUnit;
+            const uint32_t base = ring + stage * Sh::kStageBytes;
+            const uint32_t mbase = base + 2 * Sh::kCodeBytes + m_off;
+            const uint32_t badbits = (bad >> (2 * stage)) & 3u;
+            const bool masked = badbits != 0 || p0 + kPaStep - 1 > seen_all;
+
+            // ---- scores
+            float S[2][NT][4];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float D[NG][NT][4];
+                float ks[NG][2], kz[NG][2];
+#pragma unroll
+                for (int ng = 0; ng < NG; ng++) {
+                    const uint32_t addr = base + ng * (kPaStep * 32) + j * 512 + k_off;
+                    const uint2 x = lds64(addr), y = lds64(addr + 256);
+                    const uint32_t xs[2] = {x.x, x.y}, ys[2] = {y.x, y.y};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) D[ng][nt][k] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t xx = xs[e] >> (8 * h), yy = ys[e] >> (8 * h);
+                            const uint32_t a0 = xx & kEven, a1 = yy & kEven, a2 = xx & kOdd, a3 = yy & kOdd;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+                                mma_f16(D[ng][nt], a0, a1, a2, a3, q[nt][ng][2 * e + h][0], q[nt][ng][2 * e + h][1]);
+                        }
+                    const uint32_t m0 = lds32(mbase + j * (64 * NG) + 4 * ng), m1 = lds32(mbase + j * (64 * NG) + 32 * NG + 4 * ng);
+                    ks[ng][0] = meta_step(m0); kz[ng][0] = meta_low(m0);
+                    ks[ng][1] = meta_step(m1); kz[ng][1] = meta_low(m1);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        float s = 0.0f;
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++)
+                            s = fmaf(kz[ng][k >> 1], qs[nt][ng][k & 1], fmaf(ks[ng][k >> 1], D[ng][nt][k], s));
+                        S[j][nt][k] = s * cf[nt][k & 1];
+                    }
+            }
+            // positions that a column does not see; a bit a value in `off`, for the weights below
+            uint32_t off = 0;
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int p = p0 + 16 * j + tile_pos(g) + (k >> 1) * 8;
+                            if (p > lim[nt][k & 1] || ((badbits >> j) & 1u)) {
+                                S[j][nt][k] = -INFINITY;
+                                off |= 1u << ((j * NT + nt) * 4 + k);
+                            }
+                        }
+            }
+            // ---- running maximum: raised only where a score passes it by 2^8, so weights stay below 2^8
+            bool grow = false;
+            float top[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    top[nt][c] = fmaxf(fmaxf(S[0][nt][c], S[0][nt][c + 2]), fmaxf(S[1][nt][c], S[1][nt][c + 2]));
+                    grow = grow || top[nt][c] > m[nt][c] + 8.0f;
+                }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float x = top[nt][c];
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                        const float mn = fmaxf(m[nt][c], x);
+                        const float f = mn == m[nt][c] ? 1.0f : ex2(m[nt][c] - mn);
+                        m[nt][c] = mn;
+                        l[nt][c] *= f;
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++) {
+                            az[nt][ng][c] *= f;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                acc[nt][ng][i][c] *= f;
+                                acc[nt][ng][i][c + 2] *= f;
+                            }
+                        }
+                    }
+            }
+            // ---- V steps; those of positions that no column sees may be anything
+            uint32_t vm[2][NG][2];
+            int big = 0;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        uint32_t v = lds32(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG) + 4 * ng);
+                        if (masked && (p0 + 16 * j + tile_pos(g) + 8 * k >= p_end || ((badbits >> j) & 1u))) v = 0;
+                        vm[j][ng][k] = v;
+                        big = max(big, (int)(v & 0x7fffu));
+                    }
+            if (__any_sync(0xffffffffu, big > s_lim)) {
+                // a step beyond what the factor allows: take the warp's largest finite one
+                big = 0;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const int s = (int)(vm[j][ng][k] & 0x7fffu);
+                            if (s < 0x7f80) big = max(big, s);
+                        }
+                big = __reduce_max_sync(0xffffffffu, big);
+                if (big > s_lim) {
+                    const int ef = big >> 7;
+                    const int field = big == 0 ? 127 : min(258 - ef, 254);  // largest step -> [2^4, 2^5)
+                    const int d = 127 + field - s_field;
+                    const float f = d <= 0 ? 0.0f : pow2_field(min(d, 254));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++) acc[nt][ng][i][k] *= f;
+                    s_field = field;
+                    s_lim = big == 0 ? 0 : ((ef + 2) << 7) | 0x7f;  // two exponents of growth: weights below 2^15
+                }
+            }
+            const float sf = pow2_field(s_field);
+            // ---- weights: FP32 statistics, FP16 operands
+            uint32_t wb[2][NT][NG][2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float vs[NG][2], vz[NG][2];
+#pragma unroll
+                for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        vs[ng][k] = meta_step(vm[j][ng][k]) * sf;
+                        vz[ng][k] = meta_low(vm[j][ng][k]);
+                    }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float p[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float mm = m[nt][k & 1];
+                        p[k] = ex2(S[j][nt][k] - (mm == -INFINITY ? 0.0f : mm));
+                        l[nt][k & 1] += p[k];
+                    }
+#pragma unroll
+                    for (int ng = 0; ng < NG; ng++) {
+                        float x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            x[k] = p[k] * vs[ng][k >> 1];
+                            float z = p[k] * vz[ng][k >> 1];
+                            // 0 times a step that is NaN, of a position that this column does not see
+                            if (masked && ((off >> ((j * NT + nt) * 4 + k)) & 1u)) x[k] = z = 0.0f;
+                            az[nt][ng][k & 1] += z;
+                        }
+                        wb[j][nt][ng][0] = mov_trans(f16x2(x[0], x[1]));
+                        wb[j][nt][ng][1] = mov_trans(f16x2(x[2], x[3]));
+                    }
+                }
+            }
+            // ---- out += codes_V^T . weights
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int ng = 0; ng < NG; ng++) {
+                    const uint32_t vaddr = base + Sh::kCodeBytes + ng * (kPaStep * 32) + j * 512;
+                    const uint32_t x0 = lds32(vaddr + va_off), x1 = lds32(vaddr + vb_off);
+                    const uint32_t y0 = lds32(vaddr + 256 + va_off), y1 = lds32(vaddr + 256 + vb_off);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t sel = i < 2 ? 0x5410u : 0x7632u;
+                        const uint32_t x = __byte_perm(x0, x1, sel) >> (8 * (i & 1)), y = __byte_perm(y0, y1, sel) >> (8 * (i & 1));
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            mma_f16(acc[nt][ng][i], x & kEven, x & kOdd, y & kEven, y & kOdd, wb[j][nt][ng][0], wb[j][nt][ng][1]);
+                    }
+                }
+        }
+
+        // ---- join the four warps
+        float* slab = reinterpret_cast<float*>(smem);
+        float* s_m = slab + kPaWarps * COLS * Sh::kPitch;
+        float* s_l = s_m + kPaWarps * COLS;
+        cp_async_wait<0>();
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+#pragma unroll
+                    for (int ng = 0; ng < NG; ng++) az[nt][ng][c] += __shfl_xor_sync(0xffffffffu, az[nt][ng][c], o);
+                }
+                if (g == 0) s_m[w * COLS + nt * 8 + 2 * t + c] = m[nt][c];
+            }
+        __syncthreads();
+        const float unscale = pow2_field(254 - s_field);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int col = nt * 8 + 2 * t + c;
+                float M = s_m[col];
+#pragma unroll
+                for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
+                const float f = m[nt][c] == -INFINITY ? 0.0f : ex2(m[nt][c] - M);
+                if (g == 0) s_l[w * COLS + col] = m[nt][c] == -INFINITY ? l[nt][c] : l[nt][c] * f;
+                float* dst = slab + (w * COLS + col) * Sh::kPitch;
+#pragma unroll
+                for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int ch = ng * kW4Group + 8 * g + 2 * i;
+                        dst[ch] = fmaf(acc[nt][ng][i][c] * 16777216.0f, unscale, az[nt][ng][c]) * f;
+                        dst[ch + 1] = fmaf(acc[nt][ng][i][c + 2] * 1048576.0f, unscale, az[nt][ng][c]) * f;
+                    }
+            }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == rq.units;
+        float* slot = a.ws + ((size_t)blockIdx.x * 2 + (t0 > 0 ? 0 : 1)) * Sh::kSlot;
+        for (int i = tid; i < ncol * (HS / 2); i += kPaThreads) {
+            const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
+            float x = 0.0f, y = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kPaWarps; k++) {
+                x += slab[(k * COLS + col) * Sh::kPitch + ch];
+                y += slab[(k * COLS + col) * Sh::kPitch + ch + 1];
+                sum += s_l[k * COLS + col];
+            }
+            if (whole) {
+                const int gc = chunk * COLS + col;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                __nv_bfloat16* o = a.out + (size_t)(rq.r0 + gc / ratio) * a.NH * HS + (size_t)(kvh * ratio + gc % ratio) * HS + ch;
+                *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x * inv, y * inv);
+            } else {
+                slot[col * HS + ch] = x;
+                slot[col * HS + ch + 1] = y;
+                if (ch == 0) {
+                    float M = s_m[col];
+                    for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
+                    slot[COLS * HS + col] = M;
+                    slot[COLS * HS + COLS + col] = sum;
+                }
+            }
+        }
+        __syncthreads();
     }
+    pdl_trigger();
+}
+
+// Joins the pieces of the segments that several CTAs shared: block i takes the segment
+// that the border between the runs of CTAs i and i + 1 cuts, if that is the segment's
+// first border.  Pieces are added in the order of their CTAs.
+template <int NG, int NT>
+__global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnArgs a, int main_grid) {
+    using Sh = PaShape<NG, NT>;
+    constexpr int HS = Sh::kHS, COLS = Sh::kCols;
+    extern __shared__ __align__(16) unsigned char smem[];
+    long long* pre = reinterpret_cast<long long*>(smem);
+    __shared__ long long wsum[kPaWarps];
+    pa_scan(a, COLS, pre, wsum, false);
+    const long long total = pre[a.B], G = min((long long)main_grid, total);
+    const long long i0 = blockIdx.x;
+    const int ratio = a.NH / a.NKV;
+    bool mine = false;
+    int b = 0, kvh = 0, chunk = 0;
+    long long i1 = 0;
+    PaRequest rq{};
+    if (i0 + 1 < G) {
+        const long long u = total * (i0 + 1) / G;
+        b = pa_find(pre, a.B, u);
+        rq = pa_request(a, b, COLS, false);
+        const long long v = u - pre[b], per_head = (long long)rq.chunks * rq.units;
+        kvh = (int)(v / per_head);
+        chunk = (int)((v % per_head) / rq.units);
+        const long long begin = u - (v % rq.units), end = begin + rq.units;
+        // CTA of a unit x: the last one whose run begins at or before it
+        mine = begin != u && ((begin + 1) * G - 1) / total == i0;
+        i1 = (end * G - 1) / total;
+    }
+    pdl_wait();
+    if (!mine) return;
+    const int ncol = min(COLS, rq.n * ratio - chunk * COLS);
+    for (int i = blockIdx.y * kPaThreads + threadIdx.x; i < ncol * (HS / 2); i += gridDim.y * kPaThreads) {
+        const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
+        float M = -INFINITY, x = 0.0f, y = 0.0f, sum = 0.0f;
+        for (long long k = i0; k <= i1; k++) {
+            const float* slot = a.ws + ((size_t)k * 2 + (k == i0 ? 1 : 0)) * Sh::kSlot;
+            M = fmaxf(M, slot[COLS * HS + col]);
+        }
+        for (long long k = i0; k <= i1; k++) {
+            const float* slot = a.ws + ((size_t)k * 2 + (k == i0 ? 1 : 0)) * Sh::kSlot;
+            const float m = slot[COLS * HS + col];
+            const float f = m == -INFINITY ? 1.0f : ex2(m - M);  // a piece that saw nothing holds zeros (or NaN)
+            const float2 o = *reinterpret_cast<const float2*>(slot + col * HS + ch);
+            x = fmaf(o.x, f, x);
+            y = fmaf(o.y, f, y);
+            sum = fmaf(slot[COLS * HS + COLS + col], f, sum);
+        }
+        const int gc = chunk * COLS + col;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        __nv_bfloat16* o = a.out + (size_t)(rq.r0 + gc / ratio) * a.NH * HS + (size_t)(kvh * ratio + gc % ratio) * HS + ch;
+        *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x * inv, y * inv);
+    }
+}
+
+// Two tiles of 8 columns where a request's rows and shared heads give more than 8.
+static int pa_tiles(int NH, int NKV, int max_q) { return (long long)(NH / NKV) * max_q <= 8 ? 1 : 2; }
+
+template <int NG, int NT> static size_t pa_workspace() {
+    return (size_t)sm_count() * PaShape<NG, NT>::kCtas * 2 * PaShape<NG, NT>::kSlot * sizeof(float);
+}
+
+template <int NG, int NT> static cudaError_t pa_launch(const PagedAttnArgs& a, cudaStream_t st) {
+    using Sh = PaShape<NG, NT>;
+    static unsigned long long mask = 0, mask2 = 0;
+    cudaError_t e = ensure_smem_limit(paged_attn_kernel<NG, NT>, &mask);
+    if (e == cudaSuccess) e = ensure_smem_limit(paged_attn_join_kernel<NG, NT>, &mask2);
+    if (e != cudaSuccess) return e;
+    const size_t pre = sizeof(long long) * ((size_t)a.B + 1);
+    // one wave: no more CTAs than fit an SM's 228 KB of shared memory (1 KB of each is the system's)
+    const int fit = (int)(228 * 1024 / (Sh::kSmem + pre + 1024 + 64));
+    const int grid = sm_count() * (fit < Sh::kCtas ? fit : Sh::kCtas);
+    e = launch_k(paged_attn_kernel<NG, NT>, dim3(grid), dim3(kPaThreads), Sh::kSmem + pre, st, false, a);
+    if (e != cudaSuccess) return e;
+    return launch_k(paged_attn_join_kernel<NG, NT>, dim3(grid - 1, 2 * NT), dim3(kPaThreads), pre, st, true, a, grid);
 }
 
 }  // namespace gpt2b
@@ -100,7 +700,9 @@ extern "C" {
 int gpt2b_attention_paged_w4_workspace(int NH, int NKV, int hs, int max_q, size_t* bytes) {
     if (NH <= 0 || NKV <= 0 || NH % NKV != 0 || max_q <= 0 || !bytes) return GPT2B_ERR_INVALID_ARG;
     if (hs != 64 && hs != 128) return GPT2B_ERR_UNSUPPORTED;
-    *bytes = 16;
+    const int nt = pa_tiles(NH, NKV, max_q);
+    *bytes = hs == 64 ? (nt == 1 ? pa_workspace<1, 1>() : pa_workspace<1, 2>())
+                      : (nt == 1 ? pa_workspace<2, 1>() : pa_workspace<2, 2>());
     return GPT2B_OK;
 }
 
@@ -123,10 +725,13 @@ int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const u
         return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
     if ((long long)rows * NH > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
-    PagedAttnArgs a{(__nv_bfloat16*)out, (const __nv_bfloat16*)qkv, kv_cache, (const uint32_t*)kv_scale, block_table, seq_lens,
-                    row_start, B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks, scale};
-    return status_from(hs == 64 ? launch_k(paged_attn_kernel<64>, dim3(rows * NH), dim3(kPaThreads), 0, (cudaStream_t)stream, false, a)
-                                : launch_k(paged_attn_kernel<128>, dim3(rows * NH), dim3(kPaThreads), 0, (cudaStream_t)stream, false, a));
+    const PagedAttnArgs a{(__nv_bfloat16*)out, (const __nv_bfloat16*)qkv, kv_cache, (const uint32_t*)kv_scale, block_table,
+                          seq_lens, row_start, B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks,
+                          scale * 1.4426950408889634f, (float*)workspace};
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (pa_tiles(NH, NKV, max_q) == 1)
+        return status_from(hs == 64 ? pa_launch<1, 1>(a, st) : pa_launch<2, 1>(a, st));
+    return status_from(hs == 64 ? pa_launch<1, 2>(a, st) : pa_launch<2, 2>(a, st));
 }
 
 }  // extern "C"
