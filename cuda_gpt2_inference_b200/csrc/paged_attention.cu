@@ -26,6 +26,8 @@
 #include <float.h>
 #include <limits.h>
 
+#include <type_traits>
+
 namespace gpt2b {
 
 GPT2B_DEFINE_ERROR_READER(paged_attention_device_error)
@@ -37,7 +39,8 @@ struct PagedAttnArgs {
     const uint32_t* scales;
     const int *block_table, *seq_lens, *row_start;
     int B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks;
-    float scale_log2;  // softmax scale * log2(e)
+    int unit_blocks, unit_rest;  // kPaUnit in whole blocks and positions
+    float scale_log2;       // softmax scale * log2(e)
     float* ws;
 };
 
@@ -82,6 +85,21 @@ __device__ __forceinline__ PaRequest pa_request(const PagedAttnArgs& a, int b, i
     r.chunks = (r.n * (a.NH / a.NKV) + cols - 1) / cols;
     r.units = max(1, (r.len + kPaUnit - 1) / kPaUnit);  // a request that sees nothing still gets its zeros
     return r;
+}
+
+// head, tile of columns and unit of the v-th unit of a request; 32-bit divisions where they do
+struct PaPlace {
+    int kvh, chunk, unit;
+};
+__device__ __forceinline__ PaPlace pa_place(const PaRequest& r, long long v) {
+    const long long per_head = (long long)r.chunks * r.units;
+    if ((v | per_head) >> 32) {
+        const long long in = v % per_head;
+        return {(int)(v / per_head), (int)(in / r.units), (int)(in % r.units)};
+    }
+    const unsigned q = (unsigned)v / (unsigned)per_head, in = (unsigned)v - q * (unsigned)per_head;
+    const unsigned c = in / (unsigned)r.units;
+    return {(int)q, (int)c, (int)(in - c * (unsigned)r.units)};
 }
 
 // pre[b] = units of the requests before b, pre[B] = all; every thread of the CTA calls it.
@@ -159,6 +177,16 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
+// step and low end of each group of a position
+template <int NG> __device__ __forceinline__ void lds_meta(uint32_t addr, uint32_t* meta) {
+    if constexpr (NG == 1) {
+        meta[0] = lds32(addr);
+    } else {
+        const uint2 v = lds64(addr);
+        meta[0] = v.x;
+        meta[1] = v.y;
+    }
+}
 __device__ __forceinline__ float meta_step(uint32_t m) { return __uint_as_float(m << 16); }
 __device__ __forceinline__ float meta_low(uint32_t m) { return __uint_as_float(m & 0xffff0000u); }
 __device__ __forceinline__ float pow2_field(int field) { return __uint_as_float((uint32_t)field << 23); }
@@ -197,9 +225,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
     while (u < u_end) {
         while (pre[b + 1] <= u) b++;
         const PaRequest rq = pa_request(a, b, COLS, false);
-        const long long per_head = (long long)rq.chunks * rq.units, local = (u - pre[b]) % per_head;
-        const int kvh = (int)((u - pre[b]) / per_head);
-        const int chunk = (int)(local / rq.units), t0 = (int)(local % rq.units);
+        const PaPlace pl = pa_place(rq, u - pre[b]);
+        const int kvh = pl.kvh, chunk = pl.chunk, t0 = pl.unit;
         const int t1 = (int)min((long long)rq.units, t0 + (u_end - u));
         u += t1 - t0;
         const int ncol = min(COLS, rq.n * ratio - chunk * COLS);
@@ -207,6 +234,74 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         const int row_lo = chunk * COLS / ratio, row_hi = (chunk * COLS + ncol - 1) / ratio;
         const int seen_all = last + row_lo;                               // seen by every column
         const int p_end = min(min(rq.len, last + row_hi + 1), t1 * kPaUnit);  // behind the last position seen
+
+        // ---- this warp's steps: positions first + it * kPaUnit
+        const int first = t0 * kPaUnit + w * kPaStep;
+        const int steps = first < p_end ? (p_end - first + kPaUnit - 1) / kPaUnit : 0;
+        const int* table = a.block_table + (size_t)b * a.max_blocks;
+        const uint32_t head_rows = (uint32_t)a.NKV * a.block_size;  // positions of one K or V part of a block
+        const uint32_t page = head_rows * HS, meta_page = head_rows * (2 * 4 * NG);
+        const uint8_t* k_src = a.codes + (size_t)kvh * a.block_size * (HS / 2) + lane * 16;
+        const bool v_meta = lane & (4 * NG);  // lanes: [tile][K|V][16-byte piece of the tile's steps]
+        const uint8_t* m_src = reinterpret_cast<const uint8_t*>(a.scales) +
+                               ((size_t)kvh * a.block_size + (v_meta ? head_rows : 0)) * (4 * NG) + lane % (4 * NG) * 16;
+        uint32_t bad = 0;  // two bits a stage: tiles whose block lies outside the cache
+        // the next step to be issued: its place in the table, its two tiles' blocks and positions in them
+        int f_pos = first, f_idx = first / a.block_size, f_off = first % a.block_size;
+        int blk0 = 0, blk1 = 0, off0 = 0, off1 = 0;
+
+        auto fetch = [&]() {
+            if (f_pos < p_end) {
+                const bool next = f_off + 16 >= a.block_size, two = f_pos + 16 < p_end;
+                off0 = f_off;
+                off1 = two ? (next ? 0 : f_off + 16) : f_off;  // behind the end: the first tile again
+                blk0 = table[f_idx];
+                blk1 = table[f_idx + (two && next)];
+                f_pos += kPaUnit;
+                f_idx += a.unit_blocks;
+                f_off += a.unit_rest;
+                if (f_off >= a.block_size) {
+                    f_off -= a.block_size;
+                    f_idx++;
+                }
+            }
+        };
+        auto issue = [&](int it, int stage) {
+            if (it < steps) {
+                const uint32_t base = ring + stage * Sh::kStageBytes;
+                const bool bad0 = (unsigned)blk0 >= (unsigned)a.num_blocks, bad1 = (unsigned)blk1 >= (unsigned)a.num_blocks;
+                bad &= ~(3u << (2 * stage));
+                if (bad0 || bad1) {  // left out: block 0 is read in its place and masked
+                    bad |= (bad0 ? 1u : 0u) << (2 * stage) | (bad1 ? 2u : 0u) << (2 * stage);
+                    if (bad0) blk0 = 0;
+                    if (bad1) blk1 = 0;
+                    if (lane == 0) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
+                }
+                const uint8_t* src[2] = {k_src + ((size_t)(uint32_t)blk0 * page + (uint32_t)off0 * (HS / 2)),
+                                         k_src + ((size_t)(uint32_t)blk1 * page + (uint32_t)off1 * (HS / 2))};
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int k = 0; k < NG; k++) {
+                        const int i = lane + 32 * k, row = i / (2 * NG), c = i % (2 * NG);
+                        const uint32_t dst = base + (c >> 1) * (kPaStep * 32) + (16 * j + row) * 32 + (c & 1) * 16;
+                        cp_async16(dst, src[j] + k * 512);
+                        cp_async16(dst + Sh::kCodeBytes, src[j] + head_rows * (HS / 2) + k * 512);
+                    }
+                const bool hi = lane >= 8 * NG;
+                if (lane < 16 * NG)
+                    cp_async16(base + 2 * Sh::kCodeBytes + (v_meta ? Sh::kMetaBytes : 0) + (hi ? 64 * NG : 0) + lane % (4 * NG) * 16,
+                               m_src + ((size_t)(uint32_t)(hi ? blk1 : blk0) * meta_page + (uint32_t)(hi ? off1 : off0) * (4 * NG)));
+            }
+            cp_async_commit();
+        };
+
+        fetch();
+#pragma unroll
+        for (int s = 0; s < kPaStages - 1; s++) {
+            issue(s, s);
+            fetch();
+        }
 
         // ---- queries: column g of each tile as the B operand, scaled to [2^10, 2^11) at their largest
         uint32_t q[NT][NG][4][2];
@@ -234,8 +329,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const int field = min(264 - (int)(__float_as_uint(mx) >> 23), 254);
-            const float f = pow2_field(field);
-            const float c = a.scale_log2 * 1048576.0f * pow2_field(254 - field);  // D is in units of 2^-20 / f
+            // the sign of the softmax scale goes to q, so that scores grow with S
+            const float f = copysignf(pow2_field(field), a.scale_log2);
+            // D is in units of 2^-20 / f; never 0, so that a masked -infinity stays one
+            const float c = fmaxf(fabsf(a.scale_log2) * 1048576.0f * pow2_field(254 - field), 0x1p-120f);
             cf[nt][0] = __shfl_sync(0xffffffffu, c, 8 * t);
             cf[nt][1] = __shfl_sync(0xffffffffu, c, 8 * t + 4);
 #pragma unroll
@@ -271,7 +368,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         float m[NT][2], l[NT][2], az[NT][NG][2], acc[NT][NG][4][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = -INFINITY;
+            m[nt][0] = m[nt][1] = -FLT_MAX;  // nothing seen
             l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
             for (int ng = 0; ng < NG; ng++) {
@@ -282,73 +379,12 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int k = 0; k < 4; k++) acc[nt][ng][i][k] = 0.0f;
             }
         }
-        int s_lim = -1, s_field = 127;  // V steps up to s_lim (BF16 bits) fit under the factor 2^(s_field - 127)
+        float s_lim = -1.0f;  // V steps up to s_lim fit under the factor 2^(s_field - 127)
+        int s_field = 127;
 
-        // ---- this warp's steps: positions first + it * kPaUnit
-        const int first = t0 * kPaUnit + w * kPaStep;
-        const int steps = first < p_end ? (p_end - first + kPaUnit - 1) / kPaUnit : 0;
-        const int* table = a.block_table + (size_t)b * a.max_blocks;
-        uint32_t bad = 0;  // two bits a stage: tiles whose block lies outside the cache
-        int blk[2];        // the blocks of the next step to be issued
-
-        auto fetch = [&](int it) {
-            const int p = first + it * kPaUnit;
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (it < steps && p + 16 * j < p_end) blk[j] = table[(p + 16 * j) / a.block_size];
-        };
-        auto issue = [&](int it) {
-            if (it < steps) {
-                const int stage = it % kPaStages, p = first + it * kPaUnit;
-                const uint32_t base = ring + stage * Sh::kStageBytes;
-                bad &= ~(3u << (2 * stage));
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if (p + 16 * j >= p_end) continue;
-                    if (blk[j] < 0 || blk[j] >= a.num_blocks) {
-                        bad |= 1u << (2 * stage + j);
-                        if (lane == 0) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
-                        continue;
-                    }
-                    const size_t kl = (((size_t)blk[j] * 2) * a.NKV + kvh) * a.block_size + (p + 16 * j) % a.block_size;
-                    const size_t vl = kl + (size_t)a.NKV * a.block_size;
-                    const uint8_t* kc = a.codes + kl * (HS / 2);
-                    const uint8_t* vc = a.codes + vl * (HS / 2);
-#pragma unroll
-                    for (int k = 0; k < NG; k++) {
-                        const int i = lane + 32 * k, row = i / (2 * NG), c = i % (2 * NG);
-                        const uint32_t dst = base + (c >> 1) * (kPaStep * 32) + (16 * j + row) * 32 + (c & 1) * 16;
-                        cp_async16(dst, kc + i * 16);
-                        cp_async16(dst + Sh::kCodeBytes, vc + i * 16);
-                    }
-                    if (lane < 8 * NG) {
-                        const int i = lane % (4 * NG);
-                        const bool v = lane >= 4 * NG;
-                        cp_async16(base + 2 * Sh::kCodeBytes + (v ? Sh::kMetaBytes : 0) + 16 * j * 4 * NG + i * 16,
-                                   reinterpret_cast<const uint8_t*>(a.scales + (v ? vl : kl) * NG) + i * 16);
-                    }
-                }
-            }
-            cp_async_commit();
-        };
-
-        fetch(0);
-#pragma unroll
-        for (int s = 0; s < kPaStages - 1; s++) {
-            issue(s);
-            fetch(s + 1);
-        }
-        for (int it = 0; it < steps; it++) {
-            __syncwarp();  // every lane has read the stage that is filled next
-            issue(it + kPaStages - 1);
-            fetch(it + kPaStages);
-            cp_async_wait<kPaStages - 1>();
-            __syncwarp();
-            const int stage = it % kPaStages, p0 = first + it * kPaUnit;
-            const uint32_t base = ring + stage * Sh::kStageBytes;
+        auto step = [&](auto mask_tag, int p0, uint32_t base, uint32_t badbits) {
+            constexpr bool MASKED = decltype(mask_tag)::value;
             const uint32_t mbase = base + 2 * Sh::kCodeBytes + m_off;
-            const uint32_t badbits = (bad >> (2 * stage)) & 3u;
-            const bool masked = badbits != 0 || p0 + kPaStep - 1 > seen_all;
 
             // ---- scores
             float S[2][NT][4];
@@ -375,9 +411,13 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                             for (int nt = 0; nt < NT; nt++)
                                 mma_f16(D[ng][nt], a0, a1, a2, a3, q[nt][ng][2 * e + h][0], q[nt][ng][2 * e + h][1]);
                         }
-                    const uint32_t m0 = lds32(mbase + j * (64 * NG) + 4 * ng), m1 = lds32(mbase + j * (64 * NG) + 32 * NG + 4 * ng);
-                    ks[ng][0] = meta_step(m0); kz[ng][0] = meta_low(m0);
-                    ks[ng][1] = meta_step(m1); kz[ng][1] = meta_low(m1);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    uint32_t meta[NG];
+                    lds_meta<NG>(mbase + j * (64 * NG) + k * (32 * NG), meta);
+#pragma unroll
+                    for (int ng = 0; ng < NG; ng++) { ks[ng][k] = meta_step(meta[ng]); kz[ng][k] = meta_low(meta[ng]); }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -387,12 +427,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                         for (int ng = 0; ng < NG; ng++)
                             s = fmaf(kz[ng][k >> 1], qs[nt][ng][k & 1], fmaf(ks[ng][k >> 1], D[ng][nt][k], s));
-                        S[j][nt][k] = s * cf[nt][k & 1];
+                        S[j][nt][k] = s;
                     }
             }
-            // positions that a column does not see; a bit a value in `off`, for the weights below
-            uint32_t off = 0;
-            if (masked) {
+            if constexpr (MASKED) {  // positions that a column does not see
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -400,10 +438,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int p = p0 + 16 * j + tile_pos(g) + (k >> 1) * 8;
-                            if (p > lim[nt][k & 1] || ((badbits >> j) & 1u)) {
-                                S[j][nt][k] = -INFINITY;
-                                off |= 1u << ((j * NT + nt) * 4 + k);
-                            }
+                            if (p > lim[nt][k & 1] || ((badbits >> j) & 1u)) S[j][nt][k] = -INFINITY;
                         }
             }
             // ---- running maximum: raised only where a score passes it by 2^8, so weights stay below 2^8
@@ -413,7 +448,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    top[nt][c] = fmaxf(fmaxf(S[0][nt][c], S[0][nt][c + 2]), fmaxf(S[1][nt][c], S[1][nt][c + 2]));
+                    top[nt][c] = fmaxf(fmaxf(S[0][nt][c], S[0][nt][c + 2]), fmaxf(S[1][nt][c], S[1][nt][c + 2])) * cf[nt][c];
                     grow = grow || top[nt][c] > m[nt][c] + 8.0f;
                 }
             if (__any_sync(0xffffffffu, grow)) {
@@ -440,35 +475,38 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     }
             }
             // ---- V steps; those of positions that no column sees may be anything
-            uint32_t vm[2][NG][2];
-            int big = 0;
+            float vs[2][NG][2], vz[2][NG][2], big = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int ng = 0; ng < NG; ng++)
+                for (int k = 0; k < 2; k++) {
+                    uint32_t meta[NG];
+                    lds_meta<NG>(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG), meta);
+                    if (MASKED && (p0 + 16 * j + tile_pos(g) + 8 * k >= p_end || ((badbits >> j) & 1u))) {
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        uint32_t v = lds32(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG) + 4 * ng);
-                        if (masked && (p0 + 16 * j + tile_pos(g) + 8 * k >= p_end || ((badbits >> j) & 1u))) v = 0;
-                        vm[j][ng][k] = v;
-                        big = max(big, (int)(v & 0x7fffu));
+                        for (int ng = 0; ng < NG; ng++) meta[ng] = 0;
                     }
+#pragma unroll
+                    for (int ng = 0; ng < NG; ng++) {
+                        vs[j][ng][k] = meta_step(meta[ng]);
+                        vz[j][ng][k] = meta_low(meta[ng]);
+                        big = fmaxf(big, fabsf(vs[j][ng][k]));
+                    }
+                }
             if (__any_sync(0xffffffffu, big > s_lim)) {
                 // a step beyond what the factor allows: take the warp's largest finite one
-                big = 0;
+                big = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
                     for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const int s = (int)(vm[j][ng][k] & 0x7fffu);
-                            if (s < 0x7f80) big = max(big, s);
-                        }
-                big = __reduce_max_sync(0xffffffffu, big);
+                        for (int k = 0; k < 2; k++)
+                            if (fabsf(vs[j][ng][k]) < INFINITY) big = fmaxf(big, fabsf(vs[j][ng][k]));
+                big = warp_max(big);
                 if (big > s_lim) {
-                    const int ef = big >> 7;
-                    const int field = big == 0 ? 127 : min(258 - ef, 254);  // largest step -> [2^4, 2^5)
+                    const int ef = (int)(__float_as_uint(big) >> 23);
+                    const int field = big == 0.0f ? 127 : min(258 - ef, 254);  // largest step -> [2^4, 2^5)
                     const int d = 127 + field - s_field;
                     const float f = d <= 0 ? 0.0f : pow2_field(min(d, 254));
 #pragma unroll
@@ -480,7 +518,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                                 for (int k = 0; k < 4; k++) acc[nt][ng][i][k] *= f;
                     s_field = field;
-                    s_lim = big == 0 ? 0 : ((ef + 2) << 7) | 0x7f;  // two exponents of growth: weights below 2^15
+                    // up to two exponents of growth: weights stay below 2^15
+                    s_lim = big == 0.0f ? 0.0f : __uint_as_float((uint32_t)(min(ef + 2, 254)) << 23 | 0x7fffffu);
                 }
             }
             const float sf = pow2_field(s_field);
@@ -488,36 +527,45 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
             uint32_t wb[2][NT][NG][2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                float vs[NG][2], vz[NG][2];
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        vs[ng][k] = meta_step(vm[j][ng][k]) * sf;
-                        vz[ng][k] = meta_low(vm[j][ng][k]);
-                    }
+                    for (int k = 0; k < 2; k++) vs[j][ng][k] *= sf;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float p[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const float mm = m[nt][k & 1];
-                        p[k] = ex2(S[j][nt][k] - (mm == -INFINITY ? 0.0f : mm));
+                        p[k] = ex2(fmaf(S[j][nt][k], cf[nt][k & 1], -m[nt][k & 1]));
                         l[nt][k & 1] += p[k];
+                    }
+                    if constexpr (!MASKED) {
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) az[nt][ng][k & 1] = fmaf(p[k], vz[j][ng][k >> 1], az[nt][ng][k & 1]);
+                            wb[j][nt][ng][0] = f16x2(p[0] * vs[j][ng][0], p[1] * vs[j][ng][0]);
+                            wb[j][nt][ng][1] = f16x2(p[2] * vs[j][ng][1], p[3] * vs[j][ng][1]);
+                        }
+                    } else {
+                        // a position that this column does not see may hold NaN, and 0 * NaN is not 0
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++) {
+                            float x[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const bool hidden = S[j][nt][k] == -INFINITY;
+                                x[k] = hidden ? 0.0f : p[k] * vs[j][ng][k >> 1];
+                                az[nt][ng][k & 1] += hidden ? 0.0f : p[k] * vz[j][ng][k >> 1];
+                            }
+                            wb[j][nt][ng][0] = f16x2(x[0], x[1]);
+                            wb[j][nt][ng][1] = f16x2(x[2], x[3]);
+                        }
                     }
 #pragma unroll
                     for (int ng = 0; ng < NG; ng++) {
-                        float x[4];
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            x[k] = p[k] * vs[ng][k >> 1];
-                            float z = p[k] * vz[ng][k >> 1];
-                            // 0 times a step that is NaN, of a position that this column does not see
-                            if (masked && ((off >> ((j * NT + nt) * 4 + k)) & 1u)) x[k] = z = 0.0f;
-                            az[nt][ng][k & 1] += z;
-                        }
-                        wb[j][nt][ng][0] = mov_trans(f16x2(x[0], x[1]));
-                        wb[j][nt][ng][1] = mov_trans(f16x2(x[2], x[3]));
+                        wb[j][nt][ng][0] = mov_trans(wb[j][nt][ng][0]);
+                        wb[j][nt][ng][1] = mov_trans(wb[j][nt][ng][1]);
                     }
                 }
             }
@@ -538,6 +586,21 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                             mma_f16(acc[nt][ng][i], x & kEven, x & kOdd, y & kEven, y & kOdd, wb[j][nt][ng][0], wb[j][nt][ng][1]);
                     }
                 }
+        };
+        int stage = 0;
+        for (int it = 0; it < steps; it++) {
+            __syncwarp();  // every lane has read the stage that is filled next
+            issue(it + kPaStages - 1, stage == 0 ? kPaStages - 1 : stage - 1);
+            fetch();
+            cp_async_wait<kPaStages - 1>();
+            __syncwarp();
+            const int p0 = first + it * kPaUnit;
+            const uint32_t badbits = (bad >> (2 * stage)) & 3u;
+            if (badbits == 0 && p0 + kPaStep - 1 <= seen_all)
+                step(std::false_type{}, p0, ring + stage * Sh::kStageBytes, 0u);
+            else
+                step(std::true_type{}, p0, ring + stage * Sh::kStageBytes, badbits);
+            stage = stage == kPaStages - 1 ? 0 : stage + 1;
         }
 
         // ---- join the four warps
@@ -568,8 +631,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 float M = s_m[col];
 #pragma unroll
                 for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
-                const float f = m[nt][c] == -INFINITY ? 0.0f : ex2(m[nt][c] - M);
-                if (g == 0) s_l[w * COLS + col] = m[nt][c] == -INFINITY ? l[nt][c] : l[nt][c] * f;
+                const float f = ex2(m[nt][c] - M);  // 1 where nothing was seen: zeros (or NaN) are joined
+                if (g == 0) s_l[w * COLS + col] = l[nt][c] * f;
                 float* dst = slab + (w * COLS + col) * Sh::kPitch;
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++)
@@ -635,10 +698,10 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
         const long long u = total * (i0 + 1) / G;
         b = pa_find(pre, a.B, u);
         rq = pa_request(a, b, COLS, false);
-        const long long v = u - pre[b], per_head = (long long)rq.chunks * rq.units;
-        kvh = (int)(v / per_head);
-        chunk = (int)((v % per_head) / rq.units);
-        const long long begin = u - (v % rq.units), end = begin + rq.units;
+        const PaPlace pl = pa_place(rq, u - pre[b]);
+        kvh = pl.kvh;
+        chunk = pl.chunk;
+        const long long begin = u - pl.unit, end = begin + rq.units;
         // CTA of a unit x: the last one whose run begins at or before it
         mine = begin != u && ((begin + 1) * G - 1) / total == i0;
         i1 = (end * G - 1) / total;
@@ -648,7 +711,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
     const int ncol = min(COLS, rq.n * ratio - chunk * COLS);
     for (int i = blockIdx.y * kPaThreads + threadIdx.x; i < ncol * (HS / 2); i += gridDim.y * kPaThreads) {
         const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
-        float M = -INFINITY, x = 0.0f, y = 0.0f, sum = 0.0f;
+        float M = -FLT_MAX, x = 0.0f, y = 0.0f, sum = 0.0f;
         for (long long k = i0; k <= i1; k++) {
             const float* slot = a.ws + ((size_t)k * 2 + (k == i0 ? 1 : 0)) * Sh::kSlot;
             M = fmaxf(M, slot[COLS * HS + col]);
@@ -656,7 +719,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
         for (long long k = i0; k <= i1; k++) {
             const float* slot = a.ws + ((size_t)k * 2 + (k == i0 ? 1 : 0)) * Sh::kSlot;
             const float m = slot[COLS * HS + col];
-            const float f = m == -INFINITY ? 1.0f : ex2(m - M);  // a piece that saw nothing holds zeros (or NaN)
+            const float f = ex2(m - M);
             const float2 o = *reinterpret_cast<const float2*>(slot + col * HS + ch);
             x = fmaf(o.x, f, x);
             y = fmaf(o.y, f, y);
@@ -718,15 +781,18 @@ int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const u
     int rc = gpt2b_attention_paged_w4_workspace(NH, NKV, hs, max_q, &need);
     if (rc) return rc;
     if (workspace_bytes < need || ((long long)NH + 2ll * NKV) * hs > ld) return GPT2B_ERR_INVALID_ARG;
-    if (block_size % kW4Tile != 0 || B > kTableMaxRequests || (long long)max_blocks * block_size > INT_MAX)
+    // (positions are counted a few units past the end in 32 bits)
+    if (block_size % kW4Tile != 0 || B > kTableMaxRequests || (long long)max_blocks * block_size > 1 << 30)
         return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(out) || !aligned16(qkv) || !aligned16(kv_cache) || !aligned16(kv_scale) || !aligned16(workspace) ||
         ld % 8 != 0)
         return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
     if ((long long)rows * NH > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
+    if ((long long)NKV * block_size * hs > INT_MAX) return GPT2B_ERR_UNSUPPORTED;  // bytes of a block
     const PagedAttnArgs a{(__nv_bfloat16*)out, (const __nv_bfloat16*)qkv, kv_cache, (const uint32_t*)kv_scale, block_table,
                           seq_lens, row_start, B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks,
+                          kPaUnit / block_size, kPaUnit % block_size,
                           scale * 1.4426950408889634f, (float*)workspace};
     const cudaStream_t st = (cudaStream_t)stream;
     if (pa_tiles(NH, NKV, max_q) == 1)

@@ -285,7 +285,8 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
  * (1/sqrt(hs)).  max_q: the most rows a request has, a hint for the tile choice.
  * workspace: gpt2b_attention_paged_w4_workspace() bytes for the same NH, NKV, hs,
  * max_q on the current device, 16-byte aligned; needs no initialisation and holds
- * nothing between calls; calls that can overlap need one each.  B <= 4096. */
+ * nothing between calls; calls that can overlap need one each.  B <= 4096,
+ * max_blocks * block_size <= 2^30. */
 int gpt2b_attention_paged_w4_workspace(int NH, int NKV, int hs, int max_q, size_t* bytes);
 int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const uint8_t* kv_cache, const uint16_t* kv_scale,
                                      const int* block_table, const int* seq_lens, const int* row_start, int B, int rows,
