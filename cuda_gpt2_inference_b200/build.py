@@ -5,6 +5,8 @@ arch=compute_100a,code=sm_100a -lineinfo -O3 --use_fast_math``) into
 ``cuda_gpt2_inference_b200/libgpt2b.so``.  ``--use_fast_math`` matches the
 reference build (Makefile:137) so fast-math divisions in the quantisers give
 the reference's bytes.  Objects go to ``cuda_gpt2_inference_b200/_build/``.
+``csrc/bind.cpp`` (operators on torch tensors without ctypes) becomes
+``cuda_gpt2_inference_b200/_bind.so``, against the headers of the installed torch.
 
 Usage: ``python -m cuda_gpt2_inference_b200.build [--force] [--verbose] [--trace]``.
 ``--trace`` builds ``libgpt2b_trace.so`` instead (objects in ``_build_trace/``): the
@@ -17,14 +19,17 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libgpt2b.so")
+BIND = os.path.join(HERE, "_bind.so")
 OBJ_TRACE = os.path.join(HERE, "_build_trace")
 LIB_TRACE = os.path.join(HERE, "libgpt2b_trace.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
@@ -62,6 +67,15 @@ def _headers():
         glob.glob(os.path.join(INCLUDE, "*.h"))
 
 
+def _bind_command():
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    libs = os.path.join(torch, "lib")
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-I{INCLUDE}",
+            f"-I{sysconfig.get_paths()['include']}", f"-I{torch}/include", f"-I{torch}/include/torch/csrc/api/include",
+            f"-I{CUDA_HOME}/include", os.path.join(CSRC, "bind.cpp"), "-o", BIND, f"-L{libs}", "-ltorch_python",
+            "-ltorch_cpu", "-lc10_cuda", "-lc10", f"-Wl,-rpath,{libs}"]
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None, ptxas_info: bool = False,
           trace: bool = False) -> str:
     """Compile csrc/*.cu into libgpt2b.so (or the trace build) incrementally and return its path."""
@@ -74,6 +88,10 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None, p
     if trace:
         extra.append("-DGPT2B_PERSIST_TRACE=1")
     objs, work = [], []
+    bind_src = os.path.join(CSRC, "bind.cpp")
+    if not trace and (force or not os.path.exists(BIND) or os.path.getmtime(BIND) < max(
+            os.path.getmtime(bind_src), os.path.getmtime(os.path.join(INCLUDE, "gpt2_b200.h")), os.path.getmtime(__file__))):
+        work.append(_bind_command())
     for s in srcs:
         o = os.path.join(obj_dir, os.path.basename(s)[:-3] + ".o")
         objs.append(o)
@@ -88,7 +106,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None, p
     if ptxas_info:
         for o in outs:
             print(o)
-    if work or force or not os.path.exists(lib):
+    if force or not os.path.exists(lib) or any(os.path.getmtime(lib) < os.path.getmtime(o) for o in objs):
         link = [NVCC, *ARCH, "-shared", "-o", lib, *objs, "-lcudart"]
         if nccl_lib:
             link += [f"-L{nccl_lib}", "-l:libnccl.so.2", f"-Xlinker=-rpath,{nccl_lib}"]

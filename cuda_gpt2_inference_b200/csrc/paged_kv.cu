@@ -150,83 +150,145 @@ __global__ void __launch_bounds__(kTabThreads) block_tables_kernel(TableArgs a) 
 // ---------------------------------------------------------------------------
 // append and read-back
 // ---------------------------------------------------------------------------
-// 8 threads hold a group of 64 channels, 8 channels each (one 16-byte load, one
-// 4-byte store of codes); the group's ends come from three shuffles.  All sums
-// are of two terms; explicit rn operations keep the codes independent of
-// contraction and of the fast-math division.
-__global__ void __launch_bounds__(256)
-    kv_write_w4_kernel(uint8_t* codes, uint32_t* scales, const __nv_bfloat16* qkv, const long long* slot_map, int rows,
-                       int NH, int NKV, int hs, int ld, long long slots, int block_size) {
-    const int per_row = 2 * NKV * hs / 8;
-    const long long total = (long long)rows * per_row, step = (long long)gridDim.x * blockDim.x;
-    const int NG = hs / kW4Group;
-    // per_row is a multiple of 8, so the 8 threads of a group are active together
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const int row = (int)(i / per_row), c = (int)(i % per_row) * 8;
-        const uint4 v = *reinterpret_cast<const uint4*>(qkv + (size_t)row * ld + (size_t)NH * hs + c);
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 4; k++) { x[2 * k] = bf16lo(u[k]); x[2 * k + 1] = bf16hi(u[k]); }
-        float lo = x[0], hi = x[0];
-        bool fin = true;
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            lo = fminf(lo, x[k]);
-            hi = fmaxf(hi, x[k]);
-            fin = fin && (__float_as_uint(x[k]) & 0x7f800000u) != 0x7f800000u;
-        }
-        const unsigned group = 0xffu << (threadIdx.x & 24);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(group, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(group, hi, o));
-        }
-        fin = __ballot_sync(group, fin) == group;
-        uint32_t meta;
-        uint32_t word = w4_encode8(x, lo, hi, fin, meta);
-        const long long slot = slot_map[row];
-        if (slot < 0) continue;
-        if (slot >= slots) { report_device_error(GPT2B_DEVERR_BAD_BLOCK); continue; }
-        const int kv = c / (NKV * hs), h = (c / hs) % NKV, d = c % hs;
-        const size_t blk = (size_t)(slot / block_size), off = (size_t)(slot % block_size);
-        const size_t line = ((blk * 2 + kv) * NKV + h) * block_size + off;
-        *reinterpret_cast<uint32_t*>(codes + line * (hs / 2) + d / 2) = word;
-        if ((d & (kW4Group - 1)) == 0) scales[line * NG + d / kW4Group] = meta;
-    }
+// A thread holds 8 channels (one 16-byte access of BF16, one 4-byte access of codes), 8 threads a group of 64.
+// A CTA's threads cover whole rows, so a thread's head and channels are worked out once and only the slot
+// changes from row to row; each thread has kRowsAhead rows' loads in flight.
+constexpr int kRwThreads = 256, kRowsAhead = 4;
+
+struct RowPlace {
+    size_t code, meta;  // this thread's bytes in a block at offset 0
+    int row, col;       // row of the CTA's pass, channel in the row
+    bool active;
+};
+__device__ __forceinline__ RowPlace row_place(int NKV, int hs, int block_size, int per_row, int part, int parts, int rows_per_cta) {
+    RowPlace r;
+    const int i = part * kRwThreads + threadIdx.x;  // thread of the row pass, over all parts of a wide row
+    r.row = parts > 1 ? 0 : i / per_row;
+    r.col = (i - r.row * per_row) * 8;
+    r.active = parts > 1 ? i < per_row : r.row < rows_per_cta;
+    const int head = r.col / hs, d = r.col - head * hs;  // head of [K | V]
+    r.code = (size_t)head * block_size * (hs / 2) + d / 2;
+    r.meta = (size_t)head * block_size * (hs / kW4Group) + d / kW4Group;
+    return r;
+}
+struct SlotPlace {
+    size_t block;
+    int off;
+};
+__device__ __forceinline__ SlotPlace slot_place(long long slot, int block_size) {
+    if (slot >> 32) return {(size_t)(slot / block_size), (int)(slot % block_size)};
+    const unsigned b = (unsigned)slot / (unsigned)block_size;
+    return {b, (int)((unsigned)slot - b * (unsigned)block_size)};
 }
 
-__global__ void __launch_bounds__(256)
-    kv_read_w4_kernel(__nv_bfloat16* out, const uint8_t* codes, const uint32_t* scales, const long long* slot_map, int rows,
-                      int NKV, int hs, long long slots, int block_size) {
-    const int per_row = 2 * NKV * hs / 8;
-    const long long total = (long long)rows * per_row, step = (long long)gridDim.x * blockDim.x;
-    const int NG = hs / kW4Group;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const int row = (int)(i / per_row), c = (int)(i % per_row) * 8;
-        const long long slot = slot_map[row];
-        uint32_t r[4] = {0u, 0u, 0u, 0u};
-        if (slot >= slots) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
-        if (slot >= 0 && slot < slots) {
-            const int kv = c / (NKV * hs), h = (c / hs) % NKV, d = c % hs;
-            const size_t blk = (size_t)(slot / block_size), off = (size_t)(slot % block_size);
-            const size_t line = ((blk * 2 + kv) * NKV + h) * block_size + off;
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + line * (hs / 2) + d / 2);
-            const uint32_t meta = scales[line * NG + d / kW4Group];
+// Bound by HBM for many rows (rows * 2 * NKV * hs * 2.56 bytes), by its launch for few.
+__global__ void __launch_bounds__(kRwThreads)
+    kv_write_w4_kernel(uint8_t* codes, uint32_t* scales, const __nv_bfloat16* qkv, const long long* slot_map, int rows,
+                       int NH, int NKV, int hs, int ld, long long slots, int block_size, int parts, int rows_per_cta) {
+    const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
+    const RowPlace me = row_place(NKV, hs, block_size, per_row, part, parts, rows_per_cta);
+    if (!me.active) return;  // per_row is a multiple of 16: groups leave together
+    const size_t page = (size_t)NKV * block_size * hs, meta_page = page / (hs / 2) * (hs / kW4Group);
+    const long long step = (long long)(gridDim.x / parts) * rows_per_cta;
+    const __nv_bfloat16* src = qkv + (size_t)NH * hs + me.col;
+    const unsigned group = 0xffu << (threadIdx.x & 24);
+    for (long long row0 = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; row0 < rows; row0 += step * kRowsAhead) {
+        uint4 v[kRowsAhead];
+        long long slot[kRowsAhead];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const __nv_bfloat162 p = __floats2bfloat162_rn(w4_value(word, meta, 2 * k), w4_value(word, meta, 2 * k + 1));
-                r[k] = *reinterpret_cast<const uint32_t*>(&p);
+        for (int k = 0; k < kRowsAhead; k++) {
+            const long long row = row0 + k * step;
+            slot[k] = -1;
+            if (row < rows) {
+                v[k] = *reinterpret_cast<const uint4*>(src + (size_t)row * ld);
+                slot[k] = slot_map[row];
             }
         }
-        *reinterpret_cast<uint4*>(out + (size_t)row * per_row * 8 + c) = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int k = 0; k < kRowsAhead; k++) {
+            if (slot[k] < 0) continue;  // the 8 threads of a group share the row
+            if (slot[k] >= slots) {
+                report_device_error(GPT2B_DEVERR_BAD_BLOCK);
+                continue;
+            }
+            const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            // ends of the group as (min, -max): pairs, then the two halves, then 8 threads
+            uint32_t mn = bf16x2_min_nan(bf16x2_min_nan(u[0], u[1]), bf16x2_min_nan(u[2], u[3]));
+            uint32_t mx = bf16x2_min_nan(bf16x2_min_nan(u[0] ^ 0x80008000u, u[1] ^ 0x80008000u),
+                                         bf16x2_min_nan(u[2] ^ 0x80008000u, u[3] ^ 0x80008000u));
+            uint32_t e = bf16x2_min_nan(__byte_perm(mn, mx, 0x5410), __byte_perm(mn, mx, 0x7632));
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) e = bf16x2_min_nan(e, __shfl_xor_sync(group, e, o));
+            uint32_t meta;
+            const uint32_t word = w4_encode8(u, bf16lo(e), -bf16hi(e), meta);
+            const SlotPlace at = slot_place(slot[k], block_size);
+            *reinterpret_cast<uint32_t*>(codes + at.block * page + me.code + (size_t)at.off * (hs / 2)) = word;
+            if ((me.col & (kW4Group - 1)) == 0)
+                scales[at.block * meta_page + me.meta + (size_t)at.off * (hs / kW4Group)] = meta;
+        }
     }
 }
 
-// a grid of at most 8 CTAs an SM for `work` threads of 256-thread CTAs
-static int stride_grid(long long work) {
-    const long long g = (work + 255) / 256, most = (long long)sm_count() * 8;
-    return (int)(g < 1 ? 1 : (g < most ? g : most));
+__global__ void __launch_bounds__(kRwThreads)
+    kv_read_w4_kernel(__nv_bfloat16* out, const uint8_t* codes, const uint32_t* scales, const long long* slot_map, int rows,
+                      int NKV, int hs, long long slots, int block_size, int parts, int rows_per_cta) {
+    const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
+    const RowPlace me = row_place(NKV, hs, block_size, per_row, part, parts, rows_per_cta);
+    if (!me.active) return;
+    const size_t page = (size_t)NKV * block_size * hs, meta_page = page / (hs / 2) * (hs / kW4Group);
+    const long long step = (long long)(gridDim.x / parts) * rows_per_cta;
+    for (long long row0 = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; row0 < rows; row0 += step * kRowsAhead) {
+        long long slot[kRowsAhead];
+        uint32_t word[kRowsAhead], meta[kRowsAhead];
+#pragma unroll
+        for (int k = 0; k < kRowsAhead; k++) {
+            const long long row = row0 + k * step;
+            slot[k] = row < rows ? slot_map[row] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsAhead; k++) {
+            word[k] = meta[k] = 0u;  // code 0, step 0, low end 0: zeros
+            if (slot[k] >= slots) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
+            if (slot[k] >= 0 && slot[k] < slots) {
+                const SlotPlace at = slot_place(slot[k], block_size);
+                word[k] = *reinterpret_cast<const uint32_t*>(codes + at.block * page + me.code + (size_t)at.off * (hs / 2));
+                meta[k] = scales[at.block * meta_page + me.meta + (size_t)at.off * (hs / kW4Group)];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsAhead; k++) {
+            const long long row = row0 + k * step;
+            if (row >= rows) break;
+            uint32_t r[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const __nv_bfloat162 p =
+                    __floats2bfloat162_rn(w4_value(word[k], meta[k], 2 * i), w4_value(word[k], meta[k], 2 * i + 1));
+                r[i] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+            *reinterpret_cast<uint4*>(out + (size_t)row * per_row * 8 + me.col) = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+    }
+}
+
+// CTAs of a row pass: `parts` CTAs share a wide row, or a CTA takes `rows_per_cta` narrow ones; as many passes at
+// once as the rows give kRowsAhead each, at most 8 CTAs an SM.
+struct RowGrid {
+    int parts, rows_per_cta, grid;
+};
+static RowGrid row_grid(int rows, int NKV, int hs) {
+    const int per_row = 2 * NKV * hs / 8;
+    RowGrid g;
+    g.parts = (per_row + kRwThreads - 1) / kRwThreads;
+    g.rows_per_cta = g.parts > 1 ? 1 : kRwThreads / per_row;
+    // few rows: a pass each, so that all of them are on their way at once
+    long long passes = (rows + g.rows_per_cta - 1) / g.rows_per_cta;
+    const long long most = (long long)sm_count() * 8 / g.parts;
+    if (passes > most) passes = (passes + kRowsAhead - 1) / kRowsAhead;
+    if (passes > most) passes = most;
+    if (passes < 1) passes = 1;
+    g.grid = (int)(passes * g.parts);
+    return g;
 }
 
 }  // namespace gpt2b
@@ -266,17 +328,22 @@ static int w4_check(const void* codes, const void* scales, int NKV, int hs, int 
     return GPT2B_OK;
 }
 
+// the rows' channels and a block's bytes are counted in 32 bits
+static bool w4_too_large(int NKV, int hs, int block_size) { return (long long)NKV * block_size * hs > INT_MAX; }
+
 int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_t* qkv, const long long* slot_map, int rows,
                             int NH, int NKV, int hs, int ld, int num_blocks, int block_size, gpt2b_stream_t stream) {
     int rc = w4_check(kv_cache, kv_scale, NKV, hs, num_blocks, block_size);
     if (rc) return rc;
     if (rows < 0 || NH <= 0 || (rows > 0 && (!qkv || !slot_map))) return GPT2B_ERR_INVALID_ARG;
     if (((long long)NH + 2ll * NKV) * hs > ld) return GPT2B_ERR_INVALID_ARG;
+    if (w4_too_large(NKV, hs, block_size)) return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(qkv) || ld % 8 != 0) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
-    return status_from(launch_k(kv_write_w4_kernel, dim3(stride_grid((long long)rows * (2 * NKV * hs / 8))), dim3(256), 0,
-                                (cudaStream_t)stream, false, kv_cache, (uint32_t*)kv_scale, (const __nv_bfloat16*)qkv, slot_map,
-                                rows, NH, NKV, hs, ld, (long long)num_blocks * block_size, block_size));
+    const RowGrid g = row_grid(rows, NKV, hs);
+    return status_from(launch_k(kv_write_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, false, kv_cache,
+                                (uint32_t*)kv_scale, (const __nv_bfloat16*)qkv, slot_map, rows, NH, NKV, hs, ld,
+                                (long long)num_blocks * block_size, block_size, g.parts, g.rows_per_cta));
 }
 
 int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_t* kv_scale, const long long* slot_map,
@@ -284,11 +351,13 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
     int rc = w4_check(kv_cache, kv_scale, NKV, hs, num_blocks, block_size);
     if (rc) return rc;
     if (rows < 0 || (rows > 0 && (!out || !slot_map))) return GPT2B_ERR_INVALID_ARG;
+    if (w4_too_large(NKV, hs, block_size)) return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(out)) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
-    return status_from(launch_k(kv_read_w4_kernel, dim3(stride_grid((long long)rows * (2 * NKV * hs / 8))), dim3(256), 0,
-                                (cudaStream_t)stream, false, (__nv_bfloat16*)out, kv_cache, (const uint32_t*)kv_scale, slot_map,
-                                rows, NKV, hs, (long long)num_blocks * block_size, block_size));
+    const RowGrid g = row_grid(rows, NKV, hs);
+    return status_from(launch_k(kv_read_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, false,
+                                (__nv_bfloat16*)out, kv_cache, (const uint32_t*)kv_scale, slot_map, rows, NKV, hs,
+                                (long long)num_blocks * block_size, block_size, g.parts, g.rows_per_cta));
 }
 
 }  // extern "C"

@@ -10,38 +10,58 @@ constexpr int kW4Group = 64;  // channels that share a step and a low end
 constexpr int kW4Tile = 16;   // block sizes are multiples of this, so a 16-row tile lies in one block
 constexpr int kTableMaxRequests = 4096;
 
-// 8 channels of a group with ends [lo, hi] -> one word of codes; meta = step | low end << 16 (BF16 bits).
-// step = bf16(hi/15 - lo/15): each product and the difference rounded on its own, so that a range
-// beyond FP32's does not overflow.  A step below 2^-120 is held as 0 (codes 0): the division below
-// then never meets a subnormal.  The code is taken from halves for the same reason of range.
-// The step is rounded to nearest, not up: the top code then misses hi by at most 15 * 2^-9 of a step.
-// A group with a NaN or an infinity (fin false) is held as NaN.
-__device__ __forceinline__ uint32_t w4_encode8(const float* x, float lo, float hi, bool fin, uint32_t& meta) {
+// (min, -max) of BF16 pairs; NaN wins, so one NaN in a group reaches its ends
+__device__ __forceinline__ uint32_t bf16x2_min_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// 8 channels (4 BF16 pairs u) of a group with ends [lo, hi] -> one word of codes; meta = step | low end << 16
+// (BF16 bits).  step = bf16(hi/15 - lo/15): each product and the difference rounded on its own, so that a
+// range beyond FP32's does not overflow.  A step below 2^-120 is held as 0 (codes 0): the division below
+// then never meets a subnormal.  The code is taken from halves, x/2 - lo/2 over step/2, for the same reason
+// of range.  The step is rounded to nearest, not up: the top code then misses hi by at most 15 * 2^-8 of a
+// step, and no quotient reaches 15.5.  A group with a NaN or an infinity is held as NaN.
+//
+// Each code is the quotient rounded to FP32 and then to a whole number.  A product with an approximate
+// reciprocal (off by 2^-20 at most) rounds to the same number unless it comes within 2^-16 of a half: only
+// then (2^-15 of the values) the eight quotients are taken again by division.
+__device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, float hi, uint32_t& meta) {
     const float c = 1.0f / 15.0f;
-    float t = __fsub_rn(__fmul_rn(hi, c), __fmul_rn(lo, c));
-    if (t < 7.52316385e-37f) t = 0.0f;  // 2^-120
-    const uint32_t sbits = __bfloat16_as_ushort(__float2bfloat16_rn(t));
-    const float half = 0.5f * __uint_as_float(sbits << 16);
-    if (!fin) {
+    if (!(fabsf(lo) < INFINITY && fabsf(hi) < INFINITY)) {
         meta = 0x7fc07fc0u;
         return 0u;
     }
+    float t = __fsub_rn(__fmul_rn(hi, c), __fmul_rn(lo, c));
+    if (t < 0x1p-120f) t = 0.0f;
+    const uint32_t sbits = __bfloat16_as_ushort(__float2bfloat16_rn(t));
     meta = sbits | (__float_as_uint(lo) & 0xffff0000u);  // lo is a BF16 value
+    if (sbits == 0) return 0u;
+    const float half = 0.5f * __uint_as_float(sbits << 16), nlo = -0.5f * lo, inv = __fdividef(1.0f, half);
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the rounded number
+    float d[8], worst = 0.0f;
     uint32_t word = 0u;
-    if (half > 0.0f) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float d = __fsub_rn(__fmul_rn(x[k], 0.5f), __fmul_rn(lo, 0.5f));
-            const float q = fminf(rintf(__fdiv_rn(d, half)), 15.0f);
-            word |= (uint32_t)(int)q << (4 * k);
-        }
+    for (int k = 0; k < 8; k++) {
+        d[k] = fmaf(k & 1 ? bf16hi(u[k / 2]) : bf16lo(u[k / 2]), 0.5f, nlo);  // the product is exact: one rounding
+        const float q = d[k] * inv, r = __fadd_rn(q, kRound);
+        worst = fmaxf(worst, fabsf(__fsub_rn(q, __fsub_rn(r, kRound))));
+        word |= (__float_as_uint(r) & 15u) << (4 * k);
+    }
+    if (worst > 0.5f - 0x1p-16f || !(inv < 0x1p126f)) {
+        word = 0u;
+#pragma unroll
+        for (int k = 0; k < 8; k++) word |= (uint32_t)(int)rintf(__fdiv_rn(d[k], half)) << (4 * k);
     }
     return word;
 }
 
-// Channel j (0..7) of a word as FP32: code * step + low end, one rounding.
+// Channel j (0..7) of a word as FP32: code * step + low end, one rounding.  The nibble under the exponent of
+// 2^23 reads 2^23 + code.
 __device__ __forceinline__ float w4_value(uint32_t word, uint32_t meta, int j) {
-    return fmaf((float)((word >> (4 * j)) & 15u), __uint_as_float(meta << 16), __uint_as_float(meta & 0xffff0000u));
+    const float code = __uint_as_float(((word >> (4 * j)) & 15u) | 0x4b000000u) - 8388608.0f;
+    return fmaf(code, __uint_as_float(meta << 16), __uint_as_float(meta & 0xffff0000u));
 }
 
 }  // namespace gpt2b

@@ -11,13 +11,11 @@ paged 4-bit cache and for drafted tokens, at the end, have no counterpart there.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-import math
 
 import torch
 
-from . import ERR_INVALID_ARG, ERR_UNSUPPORTED, Gpt2bError, check, lib
+from . import Gpt2bError, check, lib
 
 
 def _p(t):
@@ -169,46 +167,23 @@ def gpu_argmax(d_token, logits, B, V, ld=None, stream=None):
 # ---------------------------------------------------------------------------
 # batches of requests over a paged 4-bit KV cache, and drafted tokens
 # ---------------------------------------------------------------------------
-# These take their sizes from the tensors and check them: a wrong size would
-# reach memory that is not theirs.  They run on the tensors' device (whatever the
-# current one) and, without ``stream``, on that device's current stream.
-_NULL = contextlib.nullcontext()
+# These take their sizes from the tensors and check them (a wrong size would reach
+# memory that is not theirs), run on the tensors' device whatever the current one
+# is, and without ``stream`` on that device's current stream.  The checks and the
+# call are compiled (csrc/bind.cpp): in Python they would cost more than the kernels.
+_bind = None
 
 
-def _fail(where, what, status=ERR_INVALID_ARG):
-    raise Gpt2bError(status, f"{where}: {what}")
-
-
-def _need(where, name, t, dtype, ndim, rows=False):
-    """A tensor of that type and rank, contiguous (``rows``: only within its rows)."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != ndim:
-        _fail(where, f"{name} must be a {ndim}-d {dtype} tensor")
-    if not t.is_contiguous() and not (rows and ndim == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
-        _fail(where, f"{name} must be contiguous")
-
-
-def _one_device(where, *tensors):
-    """The CUDA device that holds every tensor, as a context to call in."""
-    dev = tensors[0].device
-    if dev.type != "cuda" or any(t is not None and t.device != dev for t in tensors):
-        _fail(where, "the tensors must be on one CUDA device")
-    return dev, _NULL if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _stream_on(dev, stream):
-    return (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
-
-
-def _w4_cache(where, kv_cache, kv_scale):
-    """(num_blocks, NKV, block_size, hs) of a 4-bit cache."""
-    _need(where, "kv_cache", kv_cache, torch.uint8, 5)
-    _need(where, "kv_scale", kv_scale, torch.bfloat16, 6)
-    nb, two, NKV, bs, half = kv_cache.shape
-    if two != 2 or tuple(kv_scale.shape) != (nb, 2, NKV, bs, half // 32, 2):
-        _fail(where, "kv_cache is [blocks, 2, NKV, block_size, hs/2] and kv_scale [blocks, 2, NKV, block_size, hs/64, 2]")
-    if half not in (32, 64) or bs % 16 or bs == 0:
-        _fail(where, "head size 64 or 128, block size a multiple of 16", ERR_UNSUPPORTED)
-    return nb, NKV, bs, 2 * half
+def _b():
+    global _bind
+    if _bind is None:
+        dll = lib()
+        from . import _bind as module
+        module.init(Gpt2bError, {n: ctypes.cast(getattr(dll, n), ctypes.c_void_p).value for n in
+                                 ("gpt2b_kv_block_tables", "gpt2b_kv_cache_write_w4", "gpt2b_kv_cache_read_w4",
+                                  "gpt2b_attention_forward_paged_w4", "gpt2b_softmax_probs", "gpt2b_verify_draft_tokens")})
+        _bind = module
+    return _bind
 
 
 def kv_block_tables(block_table, slot_map, positions, row_start, seq_lens, blocks_out, free_left, ctx_lens, new_lens,
@@ -217,58 +192,23 @@ def kv_block_tables(block_table, slot_map, positions, row_start, seq_lens, block
     lengths (gpt2b_kv_block_tables).  int32, but ``slot_map`` int64; block_table
     [B, max_blocks], slot_map and positions [max_rows], row_start [B+1], free_list
     [any], free_left and free_count [1], the others [B]."""
-    w, i32 = "kv_block_tables", torch.int32
-    _need(w, "block_table", block_table, i32, 2)
-    _need(w, "slot_map", slot_map, torch.int64, 1)
-    B = block_table.shape[0]
-    for name, t, n in (("positions", positions, slot_map.shape[0]), ("row_start", row_start, B + 1),
-                       ("seq_lens", seq_lens, B), ("blocks_out", blocks_out, B), ("free_left", free_left, 1),
-                       ("ctx_lens", ctx_lens, B), ("new_lens", new_lens, B), ("blocks_have", blocks_have, B),
-                       ("free_list", free_list, None), ("free_count", free_count, 1)):
-        _need(w, name, t, i32, 1)
-        if n is not None and t.shape[0] != n:
-            _fail(w, f"{name} must have {n} entries")
-    dev, on = _one_device(w, block_table, slot_map, positions, row_start, seq_lens, blocks_out, free_left, ctx_lens, new_lens,
-                          blocks_have, free_list, free_count)
-    with on:
-        check(lib().gpt2b_kv_block_tables(block_table.data_ptr(), slot_map.data_ptr(), positions.data_ptr(),
-                                          row_start.data_ptr(), seq_lens.data_ptr(), blocks_out.data_ptr(),
-                                          free_left.data_ptr(), ctx_lens.data_ptr(), new_lens.data_ptr(),
-                                          blocks_have.data_ptr(), free_list.data_ptr(), free_count.data_ptr(), B,
-                                          block_table.shape[1], block_size, slot_map.shape[0], free_list.shape[0],
-                                          _stream_on(dev, stream)), w)
+    _b().kv_block_tables(block_table, slot_map, positions, row_start, seq_lens, blocks_out, free_left, ctx_lens, new_lens,
+                         blocks_have, free_list, free_count, block_size, stream)
 
 
 def kv_cache_write_w4(kv_cache, kv_scale, qkv, slot_map, NH, stream=None):
     """Append the K and V of packed qkv rows to the paged 4-bit cache at
-    ``slot_map`` (gpt2b_kv_cache_write_w4).  qkv BF16 [rows, >= (NH + 2 NKV) hs],
-    rows possibly further apart; slot_map int64 [rows], negative: skipped."""
-    w = "kv_cache_write_w4"
-    nb, NKV, bs, hs = _w4_cache(w, kv_cache, kv_scale)
-    _need(w, "qkv", qkv, torch.bfloat16, 2, rows=True)
-    _need(w, "slot_map", slot_map, torch.int64, 1)
-    rows, ld = qkv.shape[0], _row_pitch(qkv)
-    if slot_map.shape[0] != rows or qkv.shape[1] < (NH + 2 * NKV) * hs:
-        _fail(w, "slot_map has one entry a row, a row Q, K and V of every head")
-    dev, on = _one_device(w, kv_cache, kv_scale, qkv, slot_map)
-    with on:
-        check(lib().gpt2b_kv_cache_write_w4(kv_cache.data_ptr(), kv_scale.data_ptr(), qkv.data_ptr(), slot_map.data_ptr(), rows,
-                                            NH, NKV, hs, ld, nb, bs, _stream_on(dev, stream)), w)
+    ``slot_map`` (gpt2b_kv_cache_write_w4).  kv_cache uint8 [blocks, 2, NKV,
+    block_size, hs/2], kv_scale BF16 [blocks, 2, NKV, block_size, hs/64, 2], qkv BF16
+    [rows, >= (NH + 2 NKV) hs], rows possibly further apart; slot_map int64 [rows],
+    negative: skipped."""
+    _b().kv_cache_write_w4(kv_cache, kv_scale, qkv, slot_map, NH, stream)
 
 
 def kv_cache_read_w4(out, kv_cache, kv_scale, slot_map, stream=None):
     """Read rows of the paged 4-bit cache back as BF16 [rows, 2, NKV, hs]
     (gpt2b_kv_cache_read_w4); zeros for negative slots."""
-    w = "kv_cache_read_w4"
-    nb, NKV, bs, hs = _w4_cache(w, kv_cache, kv_scale)
-    _need(w, "out", out, torch.bfloat16, 4)
-    _need(w, "slot_map", slot_map, torch.int64, 1)
-    if tuple(out.shape) != (slot_map.shape[0], 2, NKV, hs):
-        _fail(w, "out is [rows, 2, NKV, hs]")
-    dev, on = _one_device(w, out, kv_cache, kv_scale, slot_map)
-    with on:
-        check(lib().gpt2b_kv_cache_read_w4(out.data_ptr(), kv_cache.data_ptr(), kv_scale.data_ptr(), slot_map.data_ptr(),
-                                           out.shape[0], NKV, hs, nb, bs, _stream_on(dev, stream)), w)
+    _b().kv_cache_read_w4(out, kv_cache, kv_scale, slot_map, stream)
 
 
 def attention_paged_w4_workspace(NH, NKV, hs, max_q):
@@ -281,51 +221,20 @@ def attention_paged_w4_workspace(NH, NKV, hs, max_q):
 def attention_forward_paged_w4(out, qkv, kv_cache, kv_scale, block_table, seq_lens, row_start, NH, max_q, workspace,
                                scale=None, stream=None):
     """Attention of packed rows over the paged 4-bit cache, causal among a
-    request's rows (gpt2b_attention_forward_paged_w4).  out BF16 [rows, NH hs], qkv
-    as for :func:`kv_cache_write_w4`, block_table int32 [B, max_blocks], seq_lens
+    request's rows (gpt2b_attention_forward_paged_w4).  out BF16 [rows, NH hs], cache
+    and qkv as for :func:`kv_cache_write_w4`, block_table int32 [B, max_blocks], seq_lens
     [B], row_start [B+1]; ``max_q`` the most rows a request has (a hint);
-    ``workspace`` uint8 of :func:`attention_paged_w4_workspace` bytes."""
-    w, i32 = "attention_forward_paged_w4", torch.int32
-    nb, NKV, bs, hs = _w4_cache(w, kv_cache, kv_scale)
-    _need(w, "out", out, torch.bfloat16, 2)
-    _need(w, "qkv", qkv, torch.bfloat16, 2, rows=True)
-    _need(w, "block_table", block_table, i32, 2)
-    _need(w, "seq_lens", seq_lens, i32, 1)
-    _need(w, "row_start", row_start, i32, 1)
-    _need(w, "workspace", workspace, torch.uint8, 1)
-    (rows, width), B = qkv.shape, block_table.shape[0]
-    if width < (NH + 2 * NKV) * hs or tuple(out.shape) != (rows, NH * hs):
-        _fail(w, "qkv is [rows, >= (NH + 2 NKV) hs] and out [rows, NH hs]")
-    if seq_lens.shape[0] != B or row_start.shape[0] != B + 1:
-        _fail(w, "seq_lens has B entries and row_start B + 1")
-    dev, on = _one_device(w, out, qkv, kv_cache, kv_scale, block_table, seq_lens, row_start, workspace)
-    with on:
-        check(lib().gpt2b_attention_forward_paged_w4(
-            out.data_ptr(), qkv.data_ptr(), kv_cache.data_ptr(), kv_scale.data_ptr(), block_table.data_ptr(),
-            seq_lens.data_ptr(), row_start.data_ptr(), B, rows, NH, NKV, hs, _row_pitch(qkv), nb, bs, block_table.shape[1],
-            max_q, 1.0 / math.sqrt(hs) if scale is None else scale, workspace.data_ptr(), workspace.shape[0],
-            _stream_on(dev, stream)), w)
-
-
-def _row_pitch(t):
-    """Elements between the rows of a 2-d tensor (its width where it has one row: the stride then says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    ``workspace`` uint8 of :func:`attention_paged_w4_workspace` bytes; ``scale``
+    of the scores, default 1/sqrt(hs)."""
+    _b().attention_forward_paged_w4(out, qkv, kv_cache, kv_scale, block_table, seq_lens, row_start, NH, max_q, workspace,
+                                    scale, stream)
 
 
 def softmax_probs(probs, logits, temperature=1.0, V=None, stream=None):
     """probs = softmax(logits / temperature) per row over the first ``V`` (default:
     all) columns; temperature 0: one-hot at the largest (gpt2b_softmax_probs).
     FP32 [rows, >= V]; ``probs`` may be ``logits``."""
-    w = "softmax_probs"
-    _need(w, "probs", probs, torch.float32, 2, rows=True)
-    _need(w, "logits", logits, torch.float32, 2, rows=True)
-    V = logits.shape[1] if V is None else V
-    if probs.shape[0] != logits.shape[0] or min(probs.shape[1], logits.shape[1]) < V:
-        _fail(w, "probs and logits have the same rows, of at least V columns")
-    dev, on = _one_device(w, probs, logits)
-    with on:
-        check(lib().gpt2b_softmax_probs(probs.data_ptr(), logits.data_ptr(), logits.shape[0], V, _row_pitch(logits),
-                                        _row_pitch(probs), temperature, _stream_on(dev, stream)), w)
+    _b().softmax_probs(probs, logits, temperature, V, stream)
 
 
 def verify_draft_tokens(out_tokens, n_accepted, tokens, target_probs, draft_probs, row_start, u_accept, u_sample, stream=None):
@@ -334,28 +243,4 @@ def verify_draft_tokens(out_tokens, n_accepted, tokens, target_probs, draft_prob
     n_accepted [B], tokens int32 [rows] (packed: last token, then drafts),
     target_probs FP32 [rows, V], draft_probs the same or None (certain drafts),
     row_start int32 [B+1], u_accept FP32 [rows], u_sample [B]."""
-    w, i32, f32 = "verify_draft_tokens", torch.int32, torch.float32
-    _need(w, "out_tokens", out_tokens, i32, 2)
-    _need(w, "n_accepted", n_accepted, i32, 1)
-    _need(w, "tokens", tokens, i32, 1)
-    _need(w, "target_probs", target_probs, f32, 2, rows=True)
-    _need(w, "row_start", row_start, i32, 1)
-    _need(w, "u_accept", u_accept, f32, 1)
-    _need(w, "u_sample", u_sample, f32, 1)
-    (B, max_out), (rows, V) = out_tokens.shape, target_probs.shape
-    if n_accepted.shape[0] != B or row_start.shape[0] != B + 1 or u_sample.shape[0] != B:
-        _fail(w, "n_accepted and u_sample have B entries, row_start B + 1")
-    if tokens.shape[0] != rows or u_accept.shape[0] != rows:
-        _fail(w, "tokens and u_accept have one entry a row")
-    ld_q = V
-    if draft_probs is not None:
-        _need(w, "draft_probs", draft_probs, f32, 2, rows=True)
-        if tuple(draft_probs.shape) != (rows, V):
-            _fail(w, "draft_probs has target_probs' shape")
-        ld_q = _row_pitch(draft_probs)
-    dev, on = _one_device(w, out_tokens, n_accepted, tokens, target_probs, draft_probs, row_start, u_accept, u_sample)
-    with on:
-        check(lib().gpt2b_verify_draft_tokens(out_tokens.data_ptr(), n_accepted.data_ptr(), tokens.data_ptr(),
-                                              target_probs.data_ptr(), _p(draft_probs), row_start.data_ptr(),
-                                              u_accept.data_ptr(), u_sample.data_ptr(), B, rows, V, _row_pitch(target_probs),
-                                              ld_q, max_out, _stream_on(dev, stream)), w)
+    _b().verify_draft_tokens(out_tokens, n_accepted, tokens, target_probs, draft_probs, row_start, u_accept, u_sample, stream)

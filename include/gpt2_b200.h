@@ -238,7 +238,8 @@ int gpt2b_attention_forward_kv_large_bf16_noalloc(uint16_t* out, const uint16_t*
  * A channel's value is code * s + lo.  Slot = block * block_size + offset.
  * Block tables are int32 [B][max_blocks]; entries behind a request's last block
  * are not read.  kv_cache, kv_scale, qkv and out are 16-byte aligned.
- * qkv rows are [Q (NH*hs) | K (NKV*hs) | V (NKV*hs)], ld elements apart. */
+ * qkv rows are [Q (NH*hs) | K (NKV*hs) | V (NKV*hs)], ld elements apart.
+ * A block (NKV * block_size * hs bytes of codes) is at most 2^31 - 1 bytes. */
 
 /* Block tables and row maps of one step, from the requests' lengths.  Request b
  * has ctx_lens[b] cached positions, new_lens[b] new rows (either may be 0;
