@@ -151,16 +151,17 @@ __global__ void __launch_bounds__(kTabThreads) block_tables_kernel(TableArgs a) 
 // append and read-back
 // ---------------------------------------------------------------------------
 // A thread holds 8 channels (one 16-byte access of BF16, one 4-byte access of codes), 8 threads a group of 64.
-// A CTA's threads cover whole rows, so a thread's head and channels are worked out once and only the slot
-// changes from row to row; each thread has kRowsAhead rows' loads in flight.
+// A CTA's threads cover whole rows, so a thread's head and channels are worked out once.  The 16 lanes that
+// share a row work out the places of their next 16 rows together, one each, and hand them round; a
+// row then costs a thread two shuffles and an addition of addresses.  kRowsAhead rows' loads are in flight.
 constexpr int kRwThreads = 256, kRowsAhead = 4;
 
 struct RowPlace {
-    size_t code, meta;  // this thread's bytes in a block at offset 0
-    int row, col;       // row of the CTA's pass, channel in the row
+    int row, col;  // row of the CTA's pass, channel in the row
+    size_t code;   // this thread's codes in a block, at offset 0
     bool active;
 };
-__device__ __forceinline__ RowPlace row_place(int NKV, int hs, int block_size, int per_row, int part, int parts, int rows_per_cta) {
+__device__ __forceinline__ RowPlace row_place(int hs, int block_size, int per_row, int part, int parts, int rows_per_cta) {
     RowPlace r;
     const int i = part * kRwThreads + threadIdx.x;  // thread of the row pass, over all parts of a wide row
     r.row = parts > 1 ? 0 : i / per_row;
@@ -168,17 +169,18 @@ __device__ __forceinline__ RowPlace row_place(int NKV, int hs, int block_size, i
     r.active = parts > 1 ? i < per_row : r.row < rows_per_cta;
     const int head = r.col / hs, d = r.col - head * hs;  // head of [K | V]
     r.code = (size_t)head * block_size * (hs / 2) + d / 2;
-    r.meta = (size_t)head * block_size * (hs / kW4Group) + d / kW4Group;
     return r;
 }
-struct SlotPlace {
-    size_t block;
-    int off;
-};
-__device__ __forceinline__ SlotPlace slot_place(long long slot, int block_size) {
-    if (slot >> 32) return {(size_t)(slot / block_size), (int)(slot % block_size)};
+// Byte of the codes where head 0 of the slot's row begins; -1 for no row.
+__device__ __forceinline__ long long slot_code(long long slot, long long slots, int block_size, int hs, long long page) {
+    if (slot < 0) return -1;
+    if (slot >= slots) {
+        report_device_error(GPT2B_DEVERR_BAD_BLOCK);
+        return -1;
+    }
+    if (slot >> 32) return slot / block_size * page + slot % block_size * (hs / 2);
     const unsigned b = (unsigned)slot / (unsigned)block_size;
-    return {b, (int)((unsigned)slot - b * (unsigned)block_size)};
+    return b * page + ((unsigned)slot - b * (unsigned)block_size) * (hs / 2);
 }
 
 // Bound by HBM for many rows (rows * 2 * NKV * hs * 2.56 bytes), by its launch for few.
@@ -186,45 +188,41 @@ __global__ void __launch_bounds__(kRwThreads)
     kv_write_w4_kernel(uint8_t* codes, uint32_t* scales, const __nv_bfloat16* qkv, const long long* slot_map, int rows,
                        int NH, int NKV, int hs, int ld, long long slots, int block_size, int parts, int rows_per_cta) {
     const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
-    const RowPlace me = row_place(NKV, hs, block_size, per_row, part, parts, rows_per_cta);
-    if (!me.active) return;  // per_row is a multiple of 16: groups leave together
-    const size_t page = (size_t)NKV * block_size * hs, meta_page = page / (hs / 2) * (hs / kW4Group);
-    const long long step = (long long)(gridDim.x / parts) * rows_per_cta;
+    const RowPlace me = row_place(hs, block_size, per_row, part, parts, rows_per_cta);
+    if (!me.active) return;  // per_row is a multiple of 16: the 16 lanes of a row leave together
+    const long long page = (long long)NKV * block_size * hs, step = (long long)(gridDim.x / parts) * rows_per_cta;
     const __nv_bfloat16* src = qkv + (size_t)NH * hs + me.col;
-    const unsigned group = 0xffu << (threadIdx.x & 24);
-    for (long long row0 = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; row0 < rows; row0 += step * kRowsAhead) {
-        uint4 v[kRowsAhead];
-        long long slot[kRowsAhead];
+    const unsigned sixteen = 0xffffu << (threadIdx.x & 16);
+    const bool first = (me.col & (kW4Group - 1)) == 0;
+    for (long long base = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; base < rows; base += 16 * step) {
+        const long long ahead = base + (threadIdx.x & 15) * step;
+        const long long place = ahead < rows ? slot_code(slot_map[ahead], slots, block_size, hs, page) : -1;
+        for (int k0 = 0; k0 < 16 && base + k0 * step < rows; k0 += kRowsAhead) {
+            uint4 v[kRowsAhead];
+            long long at[kRowsAhead];
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-            const long long row = row0 + k * step;
-            slot[k] = -1;
-            if (row < rows) {
-                v[k] = *reinterpret_cast<const uint4*>(src + (size_t)row * ld);
-                slot[k] = slot_map[row];
+            for (int k = 0; k < kRowsAhead; k++) {
+                const long long row = base + (k0 + k) * step;
+                at[k] = __shfl_sync(sixteen, place, k0 + k, 16);
+                if (at[k] >= 0) v[k] = *reinterpret_cast<const uint4*>(src + row * ld);
             }
-        }
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-            if (slot[k] < 0) continue;  // the 8 threads of a group share the row
-            if (slot[k] >= slots) {
-                report_device_error(GPT2B_DEVERR_BAD_BLOCK);
-                continue;
+            for (int k = 0; k < kRowsAhead; k++) {
+                if (at[k] < 0) continue;
+                const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                // ends of the group as (min, -max): pairs, then the two halves, then 8 threads
+                uint32_t mn = bf16x2_min_nan(bf16x2_min_nan(u[0], u[1]), bf16x2_min_nan(u[2], u[3]));
+                uint32_t mx = bf16x2_min_nan(bf16x2_min_nan(u[0] ^ 0x80008000u, u[1] ^ 0x80008000u),
+                                             bf16x2_min_nan(u[2] ^ 0x80008000u, u[3] ^ 0x80008000u));
+                uint32_t e = bf16x2_min_nan(__byte_perm(mn, mx, 0x5410), __byte_perm(mn, mx, 0x7632));
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) e = bf16x2_min_nan(e, __shfl_xor_sync(sixteen, e, o));
+                uint32_t meta;
+                const uint32_t word = w4_encode8(u, bf16lo(e), -bf16hi(e), meta);
+                const size_t c = (size_t)at[k] + me.code;
+                *reinterpret_cast<uint32_t*>(codes + c) = word;
+                if (first) scales[c / (kW4Group / 2)] = meta;  // a step a 32 bytes of codes, in the same order
             }
-            const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-            // ends of the group as (min, -max): pairs, then the two halves, then 8 threads
-            uint32_t mn = bf16x2_min_nan(bf16x2_min_nan(u[0], u[1]), bf16x2_min_nan(u[2], u[3]));
-            uint32_t mx = bf16x2_min_nan(bf16x2_min_nan(u[0] ^ 0x80008000u, u[1] ^ 0x80008000u),
-                                         bf16x2_min_nan(u[2] ^ 0x80008000u, u[3] ^ 0x80008000u));
-            uint32_t e = bf16x2_min_nan(__byte_perm(mn, mx, 0x5410), __byte_perm(mn, mx, 0x7632));
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) e = bf16x2_min_nan(e, __shfl_xor_sync(group, e, o));
-            uint32_t meta;
-            const uint32_t word = w4_encode8(u, bf16lo(e), -bf16hi(e), meta);
-            const SlotPlace at = slot_place(slot[k], block_size);
-            *reinterpret_cast<uint32_t*>(codes + at.block * page + me.code + (size_t)at.off * (hs / 2)) = word;
-            if ((me.col & (kW4Group - 1)) == 0)
-                scales[at.block * meta_page + me.meta + (size_t)at.off * (hs / kW4Group)] = meta;
         }
     }
 }
@@ -233,40 +231,39 @@ __global__ void __launch_bounds__(kRwThreads)
     kv_read_w4_kernel(__nv_bfloat16* out, const uint8_t* codes, const uint32_t* scales, const long long* slot_map, int rows,
                       int NKV, int hs, long long slots, int block_size, int parts, int rows_per_cta) {
     const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
-    const RowPlace me = row_place(NKV, hs, block_size, per_row, part, parts, rows_per_cta);
+    const RowPlace me = row_place(hs, block_size, per_row, part, parts, rows_per_cta);
     if (!me.active) return;
-    const size_t page = (size_t)NKV * block_size * hs, meta_page = page / (hs / 2) * (hs / kW4Group);
-    const long long step = (long long)(gridDim.x / parts) * rows_per_cta;
-    for (long long row0 = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; row0 < rows; row0 += step * kRowsAhead) {
-        long long slot[kRowsAhead];
-        uint32_t word[kRowsAhead], meta[kRowsAhead];
+    const long long page = (long long)NKV * block_size * hs, step = (long long)(gridDim.x / parts) * rows_per_cta;
+    const unsigned sixteen = 0xffffu << (threadIdx.x & 16);
+    for (long long base = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; base < rows; base += 16 * step) {
+        const long long ahead = base + (threadIdx.x & 15) * step;
+        const long long place = ahead < rows ? slot_code(slot_map[ahead], slots, block_size, hs, page) : -1;
+        for (int k0 = 0; k0 < 16 && base + k0 * step < rows; k0 += kRowsAhead) {
+            uint32_t word[kRowsAhead], meta[kRowsAhead];
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-            const long long row = row0 + k * step;
-            slot[k] = row < rows ? slot_map[row] : -1;
-        }
-#pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-            word[k] = meta[k] = 0u;  // code 0, step 0, low end 0: zeros
-            if (slot[k] >= slots) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
-            if (slot[k] >= 0 && slot[k] < slots) {
-                const SlotPlace at = slot_place(slot[k], block_size);
-                word[k] = *reinterpret_cast<const uint32_t*>(codes + at.block * page + me.code + (size_t)at.off * (hs / 2));
-                meta[k] = scales[at.block * meta_page + me.meta + (size_t)at.off * (hs / kW4Group)];
+            for (int k = 0; k < kRowsAhead; k++) {
+                const long long at = __shfl_sync(sixteen, place, k0 + k, 16);
+                word[k] = meta[k] = 0u;  // code 0, step 0, low end 0: zeros
+                if (at >= 0) {
+                    const size_t c = (size_t)at + me.code;
+                    word[k] = *reinterpret_cast<const uint32_t*>(codes + c);
+                    meta[k] = scales[c / (kW4Group / 2)];
+                }
             }
-        }
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-            const long long row = row0 + k * step;
-            if (row >= rows) break;
-            uint32_t r[4];
+            for (int k = 0; k < kRowsAhead; k++) {
+                const long long row = base + (k0 + k) * step;
+                if (row >= rows) break;
+                float x[8];
+                w4_values(word[k], meta[k], x);
+                uint32_t r[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const __nv_bfloat162 p =
-                    __floats2bfloat162_rn(w4_value(word[k], meta[k], 2 * i), w4_value(word[k], meta[k], 2 * i + 1));
-                r[i] = *reinterpret_cast<const uint32_t*>(&p);
+                for (int i = 0; i < 4; i++) {
+                    const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                    r[i] = *reinterpret_cast<const uint32_t*>(&p);
+                }
+                *reinterpret_cast<uint4*>(out + row * (per_row * 8) + me.col) = make_uint4(r[0], r[1], r[2], r[3]);
             }
-            *reinterpret_cast<uint4*>(out + (size_t)row * per_row * 8 + me.col) = make_uint4(r[0], r[1], r[2], r[3]);
         }
     }
 }

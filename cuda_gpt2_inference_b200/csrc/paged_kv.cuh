@@ -39,29 +39,38 @@ __device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, floa
     meta = sbits | (__float_as_uint(lo) & 0xffff0000u);  // lo is a BF16 value
     if (sbits == 0) return 0u;
     const float half = 0.5f * __uint_as_float(sbits << 16), nlo = -0.5f * lo, inv = __fdividef(1.0f, half);
-    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the rounded number
-    float d[8], worst = 0.0f;
-    uint32_t word = 0u;
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+    float d[8], code[8], worst = 0.0f;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
         d[k] = fmaf(k & 1 ? bf16hi(u[k / 2]) : bf16lo(u[k / 2]), 0.5f, nlo);  // the product is exact: one rounding
-        const float q = d[k] * inv, r = __fadd_rn(q, kRound);
-        worst = fmaxf(worst, fabsf(__fsub_rn(q, __fsub_rn(r, kRound))));
-        word |= (__float_as_uint(r) & 15u) << (4 * k);
+        const float q = d[k] * inv;
+        code[k] = __fsub_rn(__fadd_rn(q, kRound), kRound);
+        worst = fmaxf(worst, fabsf(__fsub_rn(q, code[k])));
     }
     if (worst > 0.5f - 0x1p-16f || !(inv < 0x1p126f)) {
-        word = 0u;
 #pragma unroll
-        for (int k = 0; k < 8; k++) word |= (uint32_t)(int)rintf(__fdiv_rn(d[k], half)) << (4 * k);
+        for (int k = 0; k < 8; k++) code[k] = rintf(__fdiv_rn(d[k], half));
     }
-    return word;
+    // four codes to a 16-bit whole number on the FMA units, its bits under the exponent of 2^23
+    float h[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        h[k] = fmaf(code[4 * k + 3], 4096.0f, fmaf(code[4 * k + 2], 256.0f, fmaf(code[4 * k + 1], 16.0f, code[4 * k]))) + 8388608.0f;
+    return __byte_perm(__float_as_uint(h[0]), __float_as_uint(h[1]), 0x5410);
 }
 
-// Channel j (0..7) of a word as FP32: code * step + low end, one rounding.  The nibble under the exponent of
-// 2^23 reads 2^23 + code.
-__device__ __forceinline__ float w4_value(uint32_t word, uint32_t meta, int j) {
-    const float code = __uint_as_float(((word >> (4 * j)) & 15u) | 0x4b000000u) - 8388608.0f;
-    return fmaf(code, __uint_as_float(meta << 16), __uint_as_float(meta & 0xffff0000u));
+// The 8 channels of a word as FP32: code * step + low end, one rounding.  Nibble k of a half, masked in place
+// under the exponent of 2^23, reads 2^23 + code * 16^k; one exact multiply-add leaves the code.
+__device__ __forceinline__ void w4_values(uint32_t word, uint32_t meta, float* x) {
+    const float s = __uint_as_float(meta << 16), lo = __uint_as_float(meta & 0xffff0000u);
+    const float down[4] = {1.0f, 0x1p-4f, 0x1p-8f, 0x1p-12f};
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const uint32_t h = k < 4 ? word : word >> 16;
+        const float f = __uint_as_float((h & (15u << (4 * (k & 3)))) | 0x4b000000u);
+        x[k] = fmaf(fmaf(f, down[k & 3], -8388608.0f * down[k & 3]), s, lo);
+    }
 }
 
 }  // namespace gpt2b

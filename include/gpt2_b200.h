@@ -339,7 +339,7 @@ int gpt2b_gpu_argmax(int* d_token, const float* logits, int B, int V, int ld, gp
 int gpt2b_logits_nll(float* d_nll, const float* logits, int V, const int* d_token, gpt2b_stream_t stream);
 
 /* probs[r] = softmax(logits[r] / temperature) over the first V logits of each
- * row (rows ld_* apart), FP32.  temperature is 0 or at least 1e-30; 0: 1 at the largest logit (lowest
+ * row (rows ld_* apart), FP32.  temperature is 0 or in [1e-30, 1e30]; 0: 1 at the largest logit (lowest
  * index on ties), 0 elsewhere.  A row with nothing above -infinity gives zeros; a
  * NaN or +infinity gives NaN (temperature 0 passes over NaN).  probs may be
  * logits.  No counterpart in the reference (its sampler keeps no probabilities). */

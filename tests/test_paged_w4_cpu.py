@@ -95,7 +95,7 @@ def test_probs_and_verify_refusals(gpt2b, mem):
     def probs(out=a, x=a, rows=1, V=8, li=8, lo=8, T=1.0):
         return lib.gpt2b_softmax_probs(out, x, rows, V, li, lo, T, None)
 
-    for bad in (dict(out=None), dict(x=None), dict(rows=-1), dict(V=0), dict(li=7), dict(lo=7), dict(T=-1.0), dict(T=nan), dict(T=1e-31),
+    for bad in (dict(out=None), dict(x=None), dict(rows=-1), dict(V=0), dict(li=7), dict(lo=7), dict(T=-1.0), dict(T=nan), dict(T=1e-31), dict(T=1e31),
                 dict(T=inf), dict(li=9)):
         assert probs(**bad) == gpt2b.ERR_INVALID_ARG, bad
     assert probs(rows=0) == gpt2b.OK
