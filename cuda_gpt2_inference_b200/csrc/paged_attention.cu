@@ -57,7 +57,11 @@ template <int NG, int NT> struct PaShape {
     static constexpr int kRing = kPaWarps * kPaStages * kStageBytes;
     static constexpr int kPitch = kHS + 1;  // floats between the columns of a warp's slab
     static constexpr int kMerge = (kPaWarps * kCols * kPitch + 2 * kPaWarps * kCols) * 4;
-    static constexpr int kSmem = ((kRing > kMerge ? kRing : kMerge) + 15) & ~15;
+    static constexpr int kJoin = ((kRing > kMerge ? kRing : kMerge) + 15) & ~15;
+    // query fragments: in registers, or where those run out in shared memory, one copy for the four warps
+    static constexpr bool kQShared = NG * NT >= 4;
+    static constexpr int kQBytes = kQShared ? NT * NG * 4 * 32 * 8 : 0;
+    static constexpr int kSmem = kJoin + kQBytes;
     static constexpr int kCtas = NG * NT <= 2 ? 4 : 3;  // resident CTAs an SM (registers)
     static constexpr int kSlot = kCols * (kHS + 2);     // floats of a partial result
 };
@@ -172,6 +176,24 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ void sts64(uint32_t addr, uint32_t x, uint32_t y) {
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+// two FP32 operations an instruction
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.ftz.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+        "add.rn.ftz.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1)
+        : "f"(a0), "f"(a1));
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
@@ -216,6 +238,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
     int b = pa_find(pre, a.B, u);
 
     // this lane's places in a stage
+    const uint32_t q_lane = smem_addr(smem) + Sh::kJoin + lane * 8;
     const uint32_t ring = smem_addr(smem) + w * (kPaStages * Sh::kStageBytes);
     const uint32_t k_off = tile_pos(g) * 32 + 8 * t;           // K codes, rows g and (+ 256) g + 8
     const uint32_t m_off = tile_pos(g) * 4 * NG;               // steps of the same rows
@@ -304,7 +327,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         }
 
         // ---- queries: column g of each tile as the B operand, scaled to [2^10, 2^11) at their largest
-        uint32_t q[NT][NG][4][2];
+        uint32_t q[Sh::kQShared ? 1 : NT][NG][4][2];
+        if constexpr (Sh::kQShared) __syncthreads();  // the piece before has been read
         float cf[NT][2], qs[NT][NG][2];
         int lim[NT][2];
 #pragma unroll
@@ -354,8 +378,13 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const float* z = v + 8 * e + 2 * h;
-                        q[nt][ng][2 * e + h][0] = f16x2(z[0] * 16.0f, z[4] * 16.0f);
-                        q[nt][ng][2 * e + h][1] = f16x2(z[1], z[5]);
+                        const uint32_t q0 = f16x2(z[0] * 16.0f, z[4] * 16.0f), q1 = f16x2(z[1], z[5]);
+                        if constexpr (Sh::kQShared) {
+                            if (w == 2 * e + h) sts64(q_lane + ((nt * NG + ng) * 4 + 2 * e + h) * 256, q0, q1);
+                        } else {
+                            q[nt][ng][2 * e + h][0] = q0;
+                            q[nt][ng][2 * e + h][1] = q1;
+                        }
                     }
             }
 #pragma unroll
@@ -364,6 +393,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 lim[nt][c2] = cc < ncol ? last + (chunk * COLS + cc) / ratio : rq.len - 1;
             }
         }
+
+        if constexpr (Sh::kQShared) __syncthreads();
 
         float m[NT][2], l[NT][2], az[NT][NG][2], acc[NT][NG][4][4];
 #pragma unroll
@@ -379,8 +410,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int k = 0; k < 4; k++) acc[nt][ng][i][k] = 0.0f;
             }
         }
-        float s_lim = -1.0f;  // V steps up to s_lim fit under the factor 2^(s_field - 127)
-        int s_field = 127;
+        // What the weights are summed with: l, az and acc carry a factor 2^s_shift that brings V's steps, as
+        // long as they do not pass s_lim, into FP16's range
+        float s_lim = -1.0f;
+        int s_shift = 0;
 
         auto step = [&](auto mask_tag, int p0, uint32_t base, uint32_t badbits) {
             constexpr bool MASKED = decltype(mask_tag)::value;
@@ -388,46 +421,55 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 
             // ---- scores
             float S[2][NT][4];
+            uint32_t km[2][2][NG];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float D[NG][NT][4];
-                float ks[NG][2], kz[NG][2];
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int ng = 0; ng < NG; ng++) {
+                for (int k = 0; k < 2; k++) lds_meta<NG>(mbase + j * (64 * NG) + k * (32 * NG), km[j][k]);
+#pragma unroll
+            for (int ng = 0; ng < NG; ng++) {
+                float D[2][NT][4];
+                uint2 x[2], y[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
                     const uint32_t addr = base + ng * (kPaStep * 32) + j * 512 + k_off;
-                    const uint2 x = lds64(addr), y = lds64(addr + 256);
-                    const uint32_t xs[2] = {x.x, x.y}, ys[2] = {y.x, y.y};
+                    x[j] = lds64(addr);
+                    y[j] = lds64(addr + 256);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) D[ng][nt][k] = 0.0f;
+                        for (int k = 0; k < 4; k++) D[j][nt][k] = 0.0f;
+                }
 #pragma unroll
-                    for (int e = 0; e < 2; e++)
+                for (int e = 0; e < 2; e++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t xx = xs[e] >> (8 * h), yy = ys[e] >> (8 * h);
+                    for (int h = 0; h < 2; h++) {
+                        uint2 qf[NT];
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            if constexpr (Sh::kQShared) qf[nt] = lds64(q_lane + ((nt * NG + ng) * 4 + 2 * e + h) * 256);
+                            else qf[nt] = make_uint2(q[nt][ng][2 * e + h][0], q[nt][ng][2 * e + h][1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const uint32_t xx = (e ? x[j].y : x[j].x) >> (8 * h), yy = (e ? y[j].y : y[j].x) >> (8 * h);
                             const uint32_t a0 = xx & kEven, a1 = yy & kEven, a2 = xx & kOdd, a3 = yy & kOdd;
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
-                                mma_f16(D[ng][nt], a0, a1, a2, a3, q[nt][ng][2 * e + h][0], q[nt][ng][2 * e + h][1]);
+                            for (int nt = 0; nt < NT; nt++) mma_f16(D[j][nt], a0, a1, a2, a3, qf[nt].x, qf[nt].y);
                         }
-                }
+                    }
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    uint32_t meta[NG];
-                    lds_meta<NG>(mbase + j * (64 * NG) + k * (32 * NG), meta);
+                for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int ng = 0; ng < NG; ng++) { ks[ng][k] = meta_step(meta[ng]); kz[ng][k] = meta_low(meta[ng]); }
-                }
+                    for (int k = 0; k < 2; k++) {
+                        const float ks = meta_step(km[j][k][ng]), kz = meta_low(km[j][k][ng]);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float s = 0.0f;
-#pragma unroll
-                        for (int ng = 0; ng < NG; ng++)
-                            s = fmaf(kz[ng][k >> 1], qs[nt][ng][k & 1], fmaf(ks[ng][k >> 1], D[ng][nt][k], s));
-                        S[j][nt][k] = s;
+                            for (int c = 0; c < 2; c++) {
+                                const float z = ng == 0 ? kz * qs[nt][0][c] : fmaf(kz, qs[nt][ng][c], S[j][nt][2 * k + c]);
+                                S[j][nt][2 * k + c] = fmaf(ks, D[j][nt][2 * k + c], z);
+                            }
                     }
             }
             if constexpr (MASKED) {  // positions that a column does not see
@@ -475,22 +517,18 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     }
             }
             // ---- V steps; those of positions that no column sees may be anything
-            float vs[2][NG][2], vz[2][NG][2], big = 0.0f;
+            uint32_t vm[2][2][NG];
+            float big = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    uint32_t meta[NG];
-                    lds_meta<NG>(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG), meta);
-                    if (MASKED && (p0 + 16 * j + tile_pos(g) + 8 * k >= p_end || ((badbits >> j) & 1u))) {
-#pragma unroll
-                        for (int ng = 0; ng < NG; ng++) meta[ng] = 0;
-                    }
+                    lds_meta<NG>(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG), vm[j][k]);
+                    const bool none = MASKED && (p0 + 16 * j + tile_pos(g) + 8 * k >= p_end || ((badbits >> j) & 1u));
 #pragma unroll
                     for (int ng = 0; ng < NG; ng++) {
-                        vs[j][ng][k] = meta_step(meta[ng]);
-                        vz[j][ng][k] = meta_low(meta[ng]);
-                        big = fmaxf(big, fabsf(vs[j][ng][k]));
+                        if (none) vm[j][k][ng] = 0;
+                        big = fmaxf(big, fabsf(meta_step(vm[j][k][ng])));
                     }
                 }
             if (__any_sync(0xffffffffu, big > s_lim)) {
@@ -501,77 +539,72 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                     for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-                        for (int k = 0; k < 2; k++)
-                            if (fabsf(vs[j][ng][k]) < INFINITY) big = fmaxf(big, fabsf(vs[j][ng][k]));
+                        for (int k = 0; k < 2; k++) {
+                            const float x = fabsf(meta_step(vm[j][k][ng]));
+                            if (x < INFINITY) big = fmaxf(big, x);
+                        }
                 big = warp_max(big);
                 if (big > s_lim) {
+                    // largest step -> [2^4, 2^5), with room for two exponents of growth: operands below 2^15.
+                    // The factor itself stays below 2^100, so that FP32 holds the sums that carry it.
                     const int ef = (int)(__float_as_uint(big) >> 23);
-                    const int field = big == 0.0f ? 127 : min(258 - ef, 254);  // largest step -> [2^4, 2^5)
-                    const int d = 127 + field - s_field;
-                    const float f = d <= 0 ? 0.0f : pow2_field(min(d, 254));
+                    const int shift = big == 0.0f ? 0 : min(131 - ef, 100);
+                    const float f = pow2_field(max(127 + shift - s_shift, 0));
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int ng = 0; ng < NG; ng++)
+                        for (int c = 0; c < 2; c++) {
+                            l[nt][c] *= f;
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
+                            for (int ng = 0; ng < NG; ng++) {
+                                az[nt][ng][c] *= f;
 #pragma unroll
-                                for (int k = 0; k < 4; k++) acc[nt][ng][i][k] *= f;
-                    s_field = field;
-                    // up to two exponents of growth: weights stay below 2^15
+                                for (int i = 0; i < 4; i++) {
+                                    acc[nt][ng][i][c] *= f;
+                                    acc[nt][ng][i][c + 2] *= f;
+                                }
+                            }
+                        }
+                    s_shift = shift;
                     s_lim = big == 0.0f ? 0.0f : __uint_as_float((uint32_t)(min(ef + 2, 254)) << 23 | 0x7fffffu);
                 }
             }
-            const float sf = pow2_field(s_field);
-            // ---- weights: FP32 statistics, FP16 operands
-            uint32_t wb[2][NT][NG][2];
+            // ---- weights (FP32 statistics, FP16 operands) and out += codes_V^T . weights
+            float off[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) off[nt][c] = (float)s_shift - m[nt][c];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-#pragma unroll
-                for (int ng = 0; ng < NG; ng++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) vs[j][ng][k] *= sf;
+                uint32_t wb[NT][NG][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float p[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        p[k] = ex2(fmaf(S[j][nt][k], cf[nt][k & 1], -m[nt][k & 1]));
-                        l[nt][k & 1] += p[k];
-                    }
-                    if constexpr (!MASKED) {
-#pragma unroll
-                        for (int ng = 0; ng < NG; ng++) {
-#pragma unroll
-                            for (int k = 0; k < 4; k++) az[nt][ng][k & 1] = fmaf(p[k], vz[j][ng][k >> 1], az[nt][ng][k & 1]);
-                            wb[j][nt][ng][0] = f16x2(p[0] * vs[j][ng][0], p[1] * vs[j][ng][0]);
-                            wb[j][nt][ng][1] = f16x2(p[2] * vs[j][ng][1], p[3] * vs[j][ng][1]);
-                        }
-                    } else {
-                        // a position that this column does not see may hold NaN, and 0 * NaN is not 0
-#pragma unroll
-                        for (int ng = 0; ng < NG; ng++) {
-                            float x[4];
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const bool hidden = S[j][nt][k] == -INFINITY;
-                                x[k] = hidden ? 0.0f : p[k] * vs[j][ng][k >> 1];
-                                az[nt][ng][k & 1] += hidden ? 0.0f : p[k] * vz[j][ng][k >> 1];
-                            }
-                            wb[j][nt][ng][0] = f16x2(x[0], x[1]);
-                            wb[j][nt][ng][1] = f16x2(x[2], x[3]);
-                        }
+                    for (int k = 0; k < 4; k += 2) {
+                        fma2(p[k], p[k + 1], S[j][nt][k], S[j][nt][k + 1], cf[nt][0], cf[nt][1], off[nt][0], off[nt][1]);
+                        p[k] = ex2(p[k]);
+                        p[k + 1] = ex2(p[k + 1]);
+                        add2(l[nt][0], l[nt][1], p[k], p[k + 1]);
                     }
 #pragma unroll
                     for (int ng = 0; ng < NG; ng++) {
-                        wb[j][nt][ng][0] = mov_trans(wb[j][nt][ng][0]);
-                        wb[j][nt][ng][1] = mov_trans(wb[j][nt][ng][1]);
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const float vs = meta_step(vm[j][k][ng]), vz = meta_low(vm[j][k][ng]);
+                            float x[2];
+#pragma unroll
+                            for (int c = 0; c < 2; c++) {
+                                // a position that this column does not see may hold NaN, and 0 * NaN is not 0
+                                const bool hidden = MASKED && S[j][nt][2 * k + c] == -INFINITY;
+                                x[c] = hidden ? 0.0f : p[2 * k + c] * vs;
+                                az[nt][ng][c] = hidden ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
+                            }
+                            wb[nt][ng][k] = mov_trans(f16x2(x[0], x[1]));
+                        }
                     }
                 }
-            }
-            // ---- out += codes_V^T . weights
-#pragma unroll
-            for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++) {
                     const uint32_t vaddr = base + Sh::kCodeBytes + ng * (kPaStep * 32) + j * 512;
@@ -583,9 +616,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                         const uint32_t x = __byte_perm(x0, x1, sel) >> (8 * (i & 1)), y = __byte_perm(y0, y1, sel) >> (8 * (i & 1));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
-                            mma_f16(acc[nt][ng][i], x & kEven, x & kOdd, y & kEven, y & kOdd, wb[j][nt][ng][0], wb[j][nt][ng][1]);
+                            mma_f16(acc[nt][ng][i], x & kEven, x & kOdd, y & kEven, y & kOdd, wb[nt][ng][0], wb[nt][ng][1]);
                     }
                 }
+            }
         };
         int stage = 0;
         for (int it = 0; it < steps; it++) {
@@ -622,7 +656,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 if (g == 0) s_m[w * COLS + nt * 8 + 2 * t + c] = m[nt][c];
             }
         __syncthreads();
-        const float unscale = pow2_field(254 - s_field);
+        const float unscale = pow2_field(127 - s_shift);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -632,15 +666,15 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                 for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
                 const float f = ex2(m[nt][c] - M);  // 1 where nothing was seen: zeros (or NaN) are joined
-                if (g == 0) s_l[w * COLS + col] = l[nt][c] * f;
+                if (g == 0) s_l[w * COLS + col] = l[nt][c] * unscale * f;
                 float* dst = slab + (w * COLS + col) * Sh::kPitch;
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int ch = ng * kW4Group + 8 * g + 2 * i;
-                        dst[ch] = fmaf(acc[nt][ng][i][c] * 16777216.0f, unscale, az[nt][ng][c]) * f;
-                        dst[ch + 1] = fmaf(acc[nt][ng][i][c + 2] * 1048576.0f, unscale, az[nt][ng][c]) * f;
+                        dst[ch] = fmaf(acc[nt][ng][i][c], 16777216.0f, az[nt][ng][c]) * unscale * f;
+                        dst[ch + 1] = fmaf(acc[nt][ng][i][c + 2], 1048576.0f, az[nt][ng][c]) * unscale * f;
                     }
             }
         __syncthreads();
