@@ -44,26 +44,26 @@ struct PagedAttnArgs {
     float* ws;
 };
 
-constexpr int kPaWarps = 4;
-constexpr int kPaThreads = 32 * kPaWarps;
-constexpr int kPaStep = 32;                     // positions a warp takes at a time
-constexpr int kPaUnit = kPaStep * kPaWarps;     // positions of a unit of the work partition
-constexpr int kPaStages = 3;                    // steps in flight a warp
+constexpr int kPaWarps = 4, kPaThreads = 32 * kPaWarps;
+constexpr int kPaStep = 32;                  // positions a warp takes at a time
+constexpr int kPaUnit = kPaStep * kPaWarps;  // positions of a unit of the work partition
 
+// NG groups of 64 channels, NT tiles of 8 columns.
 template <int NG, int NT> struct PaShape {
     static constexpr int kHS = NG * kW4Group, kCols = 8 * NT;
+    static constexpr int kStages = NG == 1 ? 3 : 2;  // steps in flight a warp
     static constexpr int kCodeBytes = kPaStep * 32 * NG, kMetaBytes = kPaStep * 4 * NG;
     static constexpr int kStageBytes = 2 * (kCodeBytes + kMetaBytes);
-    static constexpr int kRing = kPaWarps * kPaStages * kStageBytes;
+    static constexpr int kRing = kPaWarps * kStages * kStageBytes;
     static constexpr int kPitch = kHS + 1;  // floats between the columns of a warp's slab
     static constexpr int kMerge = (kPaWarps * kCols * kPitch + 2 * kPaWarps * kCols) * 4;
     static constexpr int kJoin = ((kRing > kMerge ? kRing : kMerge) + 15) & ~15;
-    // query fragments: in registers, or where those run out in shared memory, one copy for the four warps
+    // query fragments: in registers, or where those run out in shared memory, one copy for all warps
     static constexpr bool kQShared = NG * NT >= 4;
     static constexpr int kQBytes = kQShared ? NT * NG * 4 * 32 * 8 : 0;
     static constexpr int kSmem = kJoin + kQBytes;
     static constexpr int kCtas = NG * NT <= 2 ? 4 : 3;  // resident CTAs an SM (registers)
-    static constexpr int kSlot = kCols * (kHS + 2);     // floats of a partial result
+    static constexpr int kSlot = kCols * (kHS + 2);                 // floats of a partial result
 };
 
 // ---------------------------------------------------------------------------
@@ -222,13 +222,14 @@ __device__ __forceinline__ int tile_pos(int r) { return r ^ ((r >> 2) & 1); }
 template <int NG, int NT>
 __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn_kernel(PagedAttnArgs a) {
     using Sh = PaShape<NG, NT>;
-    constexpr int HS = Sh::kHS, COLS = Sh::kCols;
+    constexpr int HS = Sh::kHS, COLS = Sh::kCols, STAGES = Sh::kStages;
     extern __shared__ __align__(16) unsigned char smem[];
     long long* pre = reinterpret_cast<long long*>(smem + Sh::kSmem);
     __shared__ long long wsum[kPaWarps];
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
     const int ratio = a.NH / a.NKV;
 
+    pdl_trigger();  // the joining launch may wait on the SMs as they become free
     pa_scan(a, COLS, pre, wsum, blockIdx.x == 0);
     const long long total = pre[a.B];
     const long long G = min((long long)gridDim.x, total);
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 
     // this lane's places in a stage
     const uint32_t q_lane = smem_addr(smem) + Sh::kJoin + lane * 8;
-    const uint32_t ring = smem_addr(smem) + w * (kPaStages * Sh::kStageBytes);
+    const uint32_t ring = smem_addr(smem) + w * (STAGES * Sh::kStageBytes);
     const uint32_t k_off = tile_pos(g) * 32 + 8 * t;           // K codes, rows g and (+ 256) g + 8
     const uint32_t m_off = tile_pos(g) * 4 * NG;               // steps of the same rows
     const uint32_t va_off = tile_pos(2 * t) * 32 + 4 * g;      // V codes of the row pairs (2t, 2t + 1)
@@ -258,7 +259,22 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         const int seen_all = last + row_lo;                               // seen by every column
         const int p_end = min(min(rq.len, last + row_hi + 1), t1 * kPaUnit);  // behind the last position seen
 
-        // ---- this warp's steps: positions first + it * kPaUnit
+        // ---- queries, on their way while the first blocks are looked up: column g of each tile, channels
+        // 16t .. 16t + 15 of each group
+        uint4 raw[NT][NG][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int col = nt * 8 + g, gc = chunk * COLS + col;
+            const __nv_bfloat16* src =
+                a.qkv + (size_t)(rq.r0 + gc / ratio) * a.ld + (size_t)(kvh * ratio + gc % ratio) * HS + 16 * t;
+#pragma unroll
+            for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    raw[nt][ng][k] = col < ncol ? *reinterpret_cast<const uint4*>(src + ng * kW4Group + 8 * k) : make_uint4(0, 0, 0, 0);
+        }
+
+        // ---- this warp's steps: positions first, first + kPaUnit, ..
         const int first = t0 * kPaUnit + w * kPaStep;
         const int steps = first < p_end ? (p_end - first + kPaUnit - 1) / kPaUnit : 0;
         const int* table = a.block_table + (size_t)b * a.max_blocks;
@@ -269,17 +285,20 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         const uint8_t* m_src = reinterpret_cast<const uint8_t*>(a.scales) +
                                ((size_t)kvh * a.block_size + (v_meta ? head_rows : 0)) * (4 * NG) + lane % (4 * NG) * 16;
         uint32_t bad = 0;  // two bits a stage: tiles whose block lies outside the cache
-        // the next step to be issued: its place in the table, its two tiles' blocks and positions in them
-        int f_pos = first, f_idx = first / a.block_size, f_off = first % a.block_size;
-        int blk0 = 0, blk1 = 0, off0 = 0, off1 = 0;
 
+        // a step on its way: its two tiles' blocks and positions in them
+        struct Step {
+            int blk0, blk1, off0, off1;
+        };
+        int f_pos = first, f_idx = first / a.block_size, f_off = first % a.block_size;  // of the next one to be looked up
         auto fetch = [&]() {
+            Step f{0, 0, 0, 0};
             if (f_pos < p_end) {
                 const bool next = f_off + 16 >= a.block_size, two = f_pos + 16 < p_end;
-                off0 = f_off;
-                off1 = two ? (next ? 0 : f_off + 16) : f_off;  // behind the end: the first tile again
-                blk0 = table[f_idx];
-                blk1 = table[f_idx + (two && next)];
+                f.off0 = f_off;
+                f.off1 = two ? (next ? 0 : f_off + 16) : f_off;  // behind the end: the first tile again
+                f.blk0 = table[f_idx];
+                f.blk1 = table[f_idx + (two && next)];
                 f_pos += kPaUnit;
                 f_idx += a.unit_blocks;
                 f_off += a.unit_rest;
@@ -288,20 +307,21 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     f_idx++;
                 }
             }
+            return f;
         };
-        auto issue = [&](int it, int stage) {
+        auto issue = [&](Step f, int it, int stage) {
             if (it < steps) {
                 const uint32_t base = ring + stage * Sh::kStageBytes;
-                const bool bad0 = (unsigned)blk0 >= (unsigned)a.num_blocks, bad1 = (unsigned)blk1 >= (unsigned)a.num_blocks;
+                const bool bad0 = (unsigned)f.blk0 >= (unsigned)a.num_blocks, bad1 = (unsigned)f.blk1 >= (unsigned)a.num_blocks;
                 bad &= ~(3u << (2 * stage));
                 if (bad0 || bad1) {  // left out: block 0 is read in its place and masked
                     bad |= (bad0 ? 1u : 0u) << (2 * stage) | (bad1 ? 2u : 0u) << (2 * stage);
-                    if (bad0) blk0 = 0;
-                    if (bad1) blk1 = 0;
+                    if (bad0) f.blk0 = 0;
+                    if (bad1) f.blk1 = 0;
                     if (lane == 0) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
                 }
-                const uint8_t* src[2] = {k_src + ((size_t)(uint32_t)blk0 * page + (uint32_t)off0 * (HS / 2)),
-                                         k_src + ((size_t)(uint32_t)blk1 * page + (uint32_t)off1 * (HS / 2))};
+                const uint8_t* src[2] = {k_src + ((size_t)(uint32_t)f.blk0 * page + (uint32_t)f.off0 * (HS / 2)),
+                                         k_src + ((size_t)(uint32_t)f.blk1 * page + (uint32_t)f.off1 * (HS / 2))};
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -314,41 +334,35 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 const bool hi = lane >= 8 * NG;
                 if (lane < 16 * NG)
                     cp_async16(base + 2 * Sh::kCodeBytes + (v_meta ? Sh::kMetaBytes : 0) + (hi ? 64 * NG : 0) + lane % (4 * NG) * 16,
-                               m_src + ((size_t)(uint32_t)(hi ? blk1 : blk0) * meta_page + (uint32_t)(hi ? off1 : off0) * (4 * NG)));
+                               m_src + ((size_t)(uint32_t)(hi ? f.blk1 : f.blk0) * meta_page + (uint32_t)(hi ? f.off1 : f.off0) * (4 * NG)));
             }
             cp_async_commit();
         };
 
-        fetch();
+        // the first steps' blocks are looked up together, not one behind the other's copies
+        Step ahead[STAGES];
 #pragma unroll
-        for (int s = 0; s < kPaStages - 1; s++) {
-            issue(s, s);
-            fetch();
-        }
+        for (int k = 0; k < STAGES; k++) ahead[k] = fetch();
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; k++) issue(ahead[k], k, k);
+        Step pending = ahead[STAGES - 1];
 
-        // ---- queries: column g of each tile as the B operand, scaled to [2^10, 2^11) at their largest
+        // ---- queries as the B operand, scaled to [2^10, 2^11) at a column's largest
         uint32_t q[Sh::kQShared ? 1 : NT][NG][4][2];
         if constexpr (Sh::kQShared) __syncthreads();  // the piece before has been read
         float cf[NT][2], qs[NT][NG][2];
         int lim[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int col = nt * 8 + g;
-            uint32_t raw[NG][8];  // words 2t and 2t + 1: 16 channels
+            uint32_t u[NG][8];
             float mx = 0.0f;
-            const int gc = chunk * COLS + col;
-            const __nv_bfloat16* src = a.qkv + (size_t)(rq.r0 + gc / ratio) * a.ld + (size_t)(kvh * ratio + gc % ratio) * HS;
 #pragma unroll
             for (int ng = 0; ng < NG; ng++) {
-                uint4 x = make_uint4(0, 0, 0, 0), y = x;
-                if (col < ncol) {
-                    x = *reinterpret_cast<const uint4*>(src + ng * kW4Group + 16 * t);
-                    y = *reinterpret_cast<const uint4*>(src + ng * kW4Group + 16 * t + 8);
-                }
-                raw[ng][0] = x.x; raw[ng][1] = x.y; raw[ng][2] = x.z; raw[ng][3] = x.w;
-                raw[ng][4] = y.x; raw[ng][5] = y.y; raw[ng][6] = y.z; raw[ng][7] = y.w;
+                const uint4 x = raw[nt][ng][0], y = raw[nt][ng][1];
+                u[ng][0] = x.x; u[ng][1] = x.y; u[ng][2] = x.z; u[ng][3] = x.w;
+                u[ng][4] = y.x; u[ng][5] = y.y; u[ng][6] = y.z; u[ng][7] = y.w;
 #pragma unroll
-                for (int k = 0; k < 8; k++) mx = fmaxf(mx, fmaxf(fabsf(bf16lo(raw[ng][k])), fabsf(bf16hi(raw[ng][k]))));
+                for (int k = 0; k < 8; k++) mx = fmaxf(mx, fmaxf(fabsf(bf16lo(u[ng][k])), fabsf(bf16hi(u[ng][k]))));
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -364,8 +378,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 float v[16], s = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    v[2 * k] = bf16lo(raw[ng][k]) * f;
-                    v[2 * k + 1] = bf16hi(raw[ng][k]) * f;
+                    v[2 * k] = bf16lo(u[ng][k]) * f;
+                    v[2 * k + 1] = bf16hi(u[ng][k]) * f;
                     s += v[2 * k] + v[2 * k + 1];
                 }
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
@@ -624,9 +638,9 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         int stage = 0;
         for (int it = 0; it < steps; it++) {
             __syncwarp();  // every lane has read the stage that is filled next
-            issue(it + kPaStages - 1, stage == 0 ? kPaStages - 1 : stage - 1);
-            fetch();
-            cp_async_wait<kPaStages - 1>();
+            issue(pending, it + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+            pending = fetch();
+            cp_async_wait<STAGES - 1>();
             __syncwarp();
             const int p0 = first + it * kPaUnit;
             const uint32_t badbits = (bad >> (2 * stage)) & 3u;
@@ -634,7 +648,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 step(std::false_type{}, p0, ring + stage * Sh::kStageBytes, 0u);
             else
                 step(std::true_type{}, p0, ring + stage * Sh::kStageBytes, badbits);
-            stage = stage == kPaStages - 1 ? 0 : stage + 1;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
 
         // ---- join the four warps
@@ -663,7 +677,6 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
             for (int c = 0; c < 2; c++) {
                 const int col = nt * 8 + 2 * t + c;
                 float M = s_m[col];
-#pragma unroll
                 for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
                 const float f = ex2(m[nt][c] - M);  // 1 where nothing was seen: zeros (or NaN) are joined
                 if (g == 0) s_l[w * COLS + col] = l[nt][c] * unscale * f;
@@ -683,7 +696,6 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         for (int i = tid; i < ncol * (HS / 2); i += kPaThreads) {
             const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
             float x = 0.0f, y = 0.0f, sum = 0.0f;
-#pragma unroll
             for (int k = 0; k < kPaWarps; k++) {
                 x += slab[(k * COLS + col) * Sh::kPitch + ch];
                 y += slab[(k * COLS + col) * Sh::kPitch + ch + 1];
@@ -707,12 +719,12 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         }
         __syncthreads();
     }
-    pdl_trigger();
 }
 
-// Joins the pieces of the segments that several CTAs shared: block i takes the segment
-// that the border between the runs of CTAs i and i + 1 cuts, if that is the segment's
-// first border.  Pieces are added in the order of their CTAs.
+// Joins the pieces of the segments that several CTAs shared: block i takes the segment that the border between
+// the runs of CTAs i and i + 1 cuts, if that is the segment's first border.  A thread holds two channels of a
+// column, a warp one column; pieces are added in the order of their CTAs.  Launched early: its CTAs find their
+// segments while the last of the main ones still run.
 template <int NG, int NT>
 __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnArgs a, int main_grid) {
     using Sh = PaShape<NG, NT>;
@@ -723,10 +735,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
     pa_scan(a, COLS, pre, wsum, false);
     const long long total = pre[a.B], G = min((long long)main_grid, total);
     const long long i0 = blockIdx.x;
-    const int ratio = a.NH / a.NKV;
+    const int ratio = a.NH / a.NKV, lane = threadIdx.x & 31;
     bool mine = false;
-    int b = 0, kvh = 0, chunk = 0;
-    long long i1 = 0;
+    int b = 0, kvh = 0, chunk = 0, pieces = 0;
     PaRequest rq{};
     if (i0 + 1 < G) {
         const long long u = total * (i0 + 1) / G;
@@ -738,32 +749,40 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
         const long long begin = u - pl.unit, end = begin + rq.units;
         // CTA of a unit x: the last one whose run begins at or before it
         mine = begin != u && ((begin + 1) * G - 1) / total == i0;
-        i1 = (end * G - 1) / total;
+        pieces = (int)((end * G - 1) / total - i0) + 1;
     }
+    const int i = (int)blockIdx.y * kPaThreads + (int)threadIdx.x;
+    const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
+    mine = mine && col < min(COLS, rq.n * ratio - chunk * COLS);
     pdl_wait();
-    if (!mine) return;
-    const int ncol = min(COLS, rq.n * ratio - chunk * COLS);
-    for (int i = blockIdx.y * kPaThreads + threadIdx.x; i < ncol * (HS / 2); i += gridDim.y * kPaThreads) {
-        const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
-        float M = -FLT_MAX, x = 0.0f, y = 0.0f, sum = 0.0f;
-        for (long long k = i0; k <= i1; k++) {
-            const float* slot = a.ws + ((size_t)k * 2 + (k == i0 ? 1 : 0)) * Sh::kSlot;
-            M = fmaxf(M, slot[COLS * HS + col]);
+    if (!mine) return;  // whole warps
+    // piece k > 0 is slot 0 of CTA i0 + k, the first slot 1 of CTA i0
+    const float* first = a.ws + ((size_t)i0 * 2 + 1) * Sh::kSlot;
+    auto slot = [&](int k) { return k == 0 ? first : first + (2 * (size_t)k - 1) * Sh::kSlot; };
+    float M = -FLT_MAX, x = 0.0f, y = 0.0f, sum = 0.0f;
+    for (int k = lane; k < pieces; k += 32) M = fmaxf(M, slot(k)[COLS * HS + col]);
+    M = warp_max(M);
+    for (int k0 = 0; k0 < pieces; k0 += 32) {
+        float f = 0.0f;
+        if (k0 + lane < pieces) {
+            const float* s = slot(k0 + lane);
+            f = ex2(s[COLS * HS + col] - M);
+            sum = fmaf(s[COLS * HS + COLS + col], f, sum);
         }
-        for (long long k = i0; k <= i1; k++) {
-            const float* slot = a.ws + ((size_t)k * 2 + (k == i0 ? 1 : 0)) * Sh::kSlot;
-            const float m = slot[COLS * HS + col];
-            const float f = ex2(m - M);
-            const float2 o = *reinterpret_cast<const float2*>(slot + col * HS + ch);
-            x = fmaf(o.x, f, x);
-            y = fmaf(o.y, f, y);
-            sum = fmaf(slot[COLS * HS + COLS + col], f, sum);
+        const int n = min(32, pieces - k0);
+#pragma unroll 8
+        for (int k = 0; k < n; k++) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float2 o = *reinterpret_cast<const float2*>(slot(k0 + k) + col * HS + ch);
+            x = fmaf(o.x, fk, x);
+            y = fmaf(o.y, fk, y);
         }
-        const int gc = chunk * COLS + col;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        __nv_bfloat16* o = a.out + (size_t)(rq.r0 + gc / ratio) * a.NH * HS + (size_t)(kvh * ratio + gc % ratio) * HS + ch;
-        *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x * inv, y * inv);
     }
+    sum = warp_sum(sum);
+    const int gc = chunk * COLS + col;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    __nv_bfloat16* o = a.out + (size_t)(rq.r0 + gc / ratio) * a.NH * HS + (size_t)(kvh * ratio + gc % ratio) * HS + ch;
+    *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x * inv, y * inv);
 }
 
 // Two tiles of 8 columns where a request's rows and shared heads give more than 8.
@@ -781,11 +800,13 @@ template <int NG, int NT> static cudaError_t pa_launch(const PagedAttnArgs& a, c
     if (e != cudaSuccess) return e;
     const size_t pre = sizeof(long long) * ((size_t)a.B + 1);
     // one wave: no more CTAs than fit an SM's 228 KB of shared memory (1 KB of each is the system's)
-    const int fit = (int)(228 * 1024 / (Sh::kSmem + pre + 1024 + 64));
+    const int fit = (int)(228 * 1024 / (Sh::kSmem + pre + 1024 + 512));
     const int grid = sm_count() * (fit < Sh::kCtas ? fit : Sh::kCtas);
     e = launch_k(paged_attn_kernel<NG, NT>, dim3(grid), dim3(kPaThreads), Sh::kSmem + pre, st, false, a);
     if (e != cudaSuccess) return e;
-    return launch_k(paged_attn_join_kernel<NG, NT>, dim3(grid - 1, 2 * NT), dim3(kPaThreads), pre, st, true, a, grid);
+    // a thread two channels of a column
+    const unsigned parts = Sh::kCols * (Sh::kHS / 2) / kPaThreads;
+    return launch_k(paged_attn_join_kernel<NG, NT>, dim3(grid - 1, parts), dim3(kPaThreads), pre, st, true, a, grid);
 }
 
 }  // namespace gpt2b
