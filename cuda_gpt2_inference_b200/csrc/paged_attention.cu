@@ -62,7 +62,11 @@ template <int NG, int NT> struct PaShape {
     static constexpr bool kQShared = NG * NT >= 4;
     static constexpr int kQBytes = kQShared ? NT * NG * 4 * 32 * 8 : 0;
     static constexpr int kSmem = kJoin + kQBytes;
-    static constexpr int kCtas = NG * NT <= 2 ? 4 : 3;  // resident CTAs an SM (registers)
+    // Resident CTAs an SM.  More registers a thread (more products in flight) beat more warps: hs 128 with 8
+    // columns (32 x 16384 positions) 3 CTAs 131 us, 4 139; hs 64 with 16 columns 3 CTAs 157, 4 172; hs 128 with 16
+    // columns 2 CTAs 183, 3 191; hs 64 with 8 columns the same for long requests, and 4 better for short ones
+    // (18.5 against 19.4 us at 16 x 1024).
+    static constexpr int kCtas = NG * NT == 1 ? 4 : NG * NT == 2 ? 3 : 2;
     static constexpr int kSlot = kCols * (kHS + 2);                 // floats of a partial result
 };
 
