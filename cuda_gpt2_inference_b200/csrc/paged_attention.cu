@@ -47,6 +47,7 @@ struct PagedAttnArgs {
 constexpr int kPaWarps = 4, kPaThreads = 32 * kPaWarps;
 constexpr int kPaStep = 32;                  // positions a warp takes at a time
 constexpr int kPaUnit = kPaStep * kPaWarps;  // positions of a unit of the work partition
+constexpr int kPaExtra = 2;                  // what a segment costs beside its units, in units
 
 // NG groups of 64 channels, NT tiles of 8 columns.
 template <int NG, int NT> struct PaShape {
@@ -74,13 +75,14 @@ template <int NG, int NT> struct PaShape {
 // work partition
 // ---------------------------------------------------------------------------
 // A segment is a (request, key/value head, tile of columns); it has ceil(len/128)
-// units.  The units of all segments are numbered in one row and dealt out in equal
-// contiguous runs to the resident CTAs, whatever the lengths are: a long request is
-// split over many CTAs, short ones share one.  A CTA writes a finished segment to
-// `out`, and the piece of a segment that it shares with its neighbours to one of its
-// two slots (0: the segment began before its run, 1: it goes on behind it).
+// units, and before them kPaExtra that stand for what it takes to begin and to end one.
+// The units of all segments are numbered in one row and dealt out in equal contiguous
+// runs to the resident CTAs, whatever the lengths are: a long request is split over
+// many CTAs, short ones share one.  A CTA writes a finished segment to `out`, and the
+// piece of a segment that it shares with its neighbours to one of its two slots (0: the
+// segment began before its run, 1: it goes on behind it).
 struct PaRequest {
-    int r0, n, len, chunks, units;
+    int r0, n, len, chunks, units;  // units with the extra ones
 };
 __device__ __forceinline__ PaRequest pa_request(const PagedAttnArgs& a, int b, int cols, bool report) {
     PaRequest r;
@@ -91,7 +93,7 @@ __device__ __forceinline__ PaRequest pa_request(const PagedAttnArgs& a, int b, i
     r.len = min(max(l0, 0), a.max_blocks * a.block_size);
     if (report && (r.r0 != s0 || r1 != s1 || l0 > r.len)) report_device_error(GPT2B_DEVERR_BAD_POS);
     r.chunks = (r.n * (a.NH / a.NKV) + cols - 1) / cols;
-    r.units = max(1, (r.len + kPaUnit - 1) / kPaUnit);  // a request that sees nothing still gets its zeros
+    r.units = kPaExtra + max(1, (r.len + kPaUnit - 1) / kPaUnit);  // a request that sees nothing still gets its zeros
     return r;
 }
 
@@ -254,9 +256,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         while (pre[b + 1] <= u) b++;
         const PaRequest rq = pa_request(a, b, COLS, false);
         const PaPlace pl = pa_place(rq, u - pre[b]);
-        const int kvh = pl.kvh, chunk = pl.chunk, t0 = pl.unit;
-        const int t1 = (int)min((long long)rq.units, t0 + (u_end - u));
-        u += t1 - t0;
+        const int kvh = pl.kvh, chunk = pl.chunk, v1 = (int)min((long long)rq.units, pl.unit + (u_end - u));
+        u += v1 - pl.unit;
+        const int t0 = max(pl.unit - kPaExtra, 0), t1 = v1 - kPaExtra;
+        if (t1 <= 0) continue;  // the next CTA begins this one
         const int ncol = min(COLS, rq.n * ratio - chunk * COLS);
         const int last = rq.len - rq.n;  // row i sees positions <= last + i
         const int row_lo = chunk * COLS / ratio, row_hi = (chunk * COLS + ncol - 1) / ratio;
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     }
             }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == rq.units;
+        const bool whole = t0 == 0 && v1 == rq.units;
         float* slot = a.ws + ((size_t)blockIdx.x * 2 + (t0 > 0 ? 0 : 1)) * Sh::kSlot;
         for (int i = tid; i < ncol * (HS / 2); i += kPaThreads) {
             const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
@@ -750,9 +753,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
         const PaPlace pl = pa_place(rq, u - pre[b]);
         kvh = pl.kvh;
         chunk = pl.chunk;
-        const long long begin = u - pl.unit, end = begin + rq.units;
+        const long long begin = u - pl.unit + kPaExtra, end = u - pl.unit + rq.units;
         // CTA of a unit x: the last one whose run begins at or before it
-        mine = begin != u && ((begin + 1) * G - 1) / total == i0;
+        mine = u > begin && ((begin + 1) * G - 1) / total == i0;
         pieces = (int)((end * G - 1) / total - i0) + 1;
     }
     const int i = (int)blockIdx.y * kPaThreads + (int)threadIdx.x;
