@@ -24,9 +24,10 @@ __device__ __forceinline__ uint32_t bf16x2_min_nan(uint32_t a, uint32_t b) {
 // of range.  The step is rounded to nearest, not up: the top code then misses hi by at most 15 * 2^-8 of a
 // step, and no quotient reaches 15.5.  A group with a NaN or an infinity is held as NaN.
 //
-// Each code is the quotient rounded to FP32 and then to a whole number.  A product with an approximate
-// reciprocal (off by 2^-20 at most) rounds to the same number unless it comes within 2^-16 of a half: only
-// then (2^-15 of the values) the eight quotients are taken again by division.
+// Each code is the quotient rounded to the nearest whole number, ties to even.  A product with an approximate
+// reciprocal (off by 2^-20 of it at most) rounds to the same number unless it comes within 2^-16 of a half.
+// Where one of the eight does (BF16 values of one binade over a step of few bits tie often), each is put right
+// by its remainder d - code * step/2, which is exact: both products have at most 24 bits above d's last.
 __device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, float hi, uint32_t& meta) {
     const float c = 1.0f / 15.0f;
     if (!(fabsf(lo) < INFINITY && fabsf(hi) < INFINITY)) {
@@ -38,7 +39,7 @@ __device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, floa
     const uint32_t sbits = __bfloat16_as_ushort(__float2bfloat16_rn(t));
     meta = sbits | (__float_as_uint(lo) & 0xffff0000u);  // lo is a BF16 value
     if (sbits == 0) return 0u;
-    const float half = 0.5f * __uint_as_float(sbits << 16), nlo = -0.5f * lo, inv = __fdividef(1.0f, half);
+    const float half = 0.5f * __uint_as_float(sbits << 16), nlo = -0.5f * lo, inv = __frcp_rn(half);
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
     float d[8], code[8], worst = 0.0f;
 #pragma unroll
@@ -48,9 +49,13 @@ __device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, floa
         code[k] = __fsub_rn(__fadd_rn(q, kRound), kRound);
         worst = fmaxf(worst, fabsf(__fsub_rn(q, code[k])));
     }
-    if (worst > 0.5f - 0x1p-16f || !(inv < 0x1p126f)) {
+    if (worst > 0.5f - 0x1p-16f) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) code[k] = rintf(__fdiv_rn(d[k], half));
+        for (int k = 0; k < 8; k++) {
+            const float e = fmaf(-code[k], half, d[k]), twice = fabsf(e + e);
+            const bool odd = code[k] != 2.0f * rintf(0.5f * code[k]);
+            if (twice > half || (twice == half && odd)) code[k] += copysignf(1.0f, e);
+        }
     }
     // four codes to a 16-bit whole number on the FMA units, its bits under the exponent of 2^23
     float h[2];

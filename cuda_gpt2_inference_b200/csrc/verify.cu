@@ -69,11 +69,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // One CTA of a row's cluster takes a contiguous part of it, R entries a thread in registers (entries beyond
-// threads * R are read twice more).  Each CTA sums e^((x - m)/T) about its own maximum m; the pairs (m, sum) are
+// 512 R are read twice more).  Each CTA sums e^((x - m)/T) about its own maximum m; the pairs (m, sum) are
 // exchanged behind the cluster's one barrier, and what a CTA holds about m is put right by one factor,
 // e^((m - M)/T) / total.  320 x 50257: 8 bytes an entry from and to HBM bound it; 5 rows: the chain launch - load
 // - exchange - store.
-constexpr int kProbThreads = 512;  // at most
+constexpr int kProbThreads = 512, kProbWarps = kProbThreads / 32;
 
 struct ProbPart {
     float m, s;
@@ -91,11 +91,12 @@ __device__ __forceinline__ void first_max(float& m, int& at) {
 template <int R>
 __global__ void __launch_bounds__(kProbThreads, R <= 16 ? 3 : 2)
     softmax_probs_kernel(float* probs, const float* logits, int V, long long ld_in, long long ld_out, bool greedy, ExpScale c) {
-    __shared__ float wm[kProbThreads / 32], wsum[kProbThreads / 32];
+    __shared__ float wm[kProbWarps], wsum[kProbWarps];
     __shared__ ProbPart all[8];
     cluster_begin();
     cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), T = (int)blockDim.x;
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    constexpr int T = kProbThreads;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     const long long row = blockIdx.x / C;
     const int share = (V + C - 1) / C, lo = min(rank * share, V), n = min(share, V - lo);
@@ -104,32 +105,34 @@ __global__ void __launch_bounds__(kProbThreads, R <= 16 ? 3 : 2)
 
     // entries in registers; -infinity behind the end.  NaN goes through the maximum.
     float v[R], m = -INFINITY;
+    const int left = n - tid;  // entry k is there while k T < left
+    x += tid;
+    out += tid;
 #pragma unroll
-    for (int k = 0; k < R; k++) v[k] = tid + k * T < n ? x[tid + k * T] : -INFINITY;
+    for (int k = 0; k < R; k++) v[k] = k * T < left ? x[k * T] : -INFINITY;
 #pragma unroll
     for (int k = 0; k < R; k++) m = max_nan(m, v[k]);
-    for (int i = tid + R * T; i < n; i += T) m = max_nan(m, x[i]);
+    for (int i = R * T; i < left; i += T) m = max_nan(m, x[i]);
 
     if (greedy) {  // the first largest, NaN left out
         m = -INFINITY;
         int at = INT_MAX;
-        for (int i = tid; i < n; i += T)
-            if (x[i] > m) { m = x[i]; at = lo + i; }
+        for (int i = 0; i < left; i += T)
+            if (x[i] > m) { m = x[i]; at = lo + tid + i; }
         first_max(m, at);
         cluster_wait();
-        __shared__ ProbPart first[8 * (kProbThreads / 32)];
-        if (lane < C) *cl.map_shared_rank(&first[rank * (kProbThreads / 32) + w], lane) = ProbPart{m, 0.0f, at, 0};
+        __shared__ ProbPart first[8 * kProbWarps];
+        if (lane < C) *cl.map_shared_rank(&first[rank * kProbWarps + w], lane) = ProbPart{m, 0.0f, at, 0};
         cluster_arrive();
         cluster_wait();
         m = -INFINITY;
         at = INT_MAX;
-        for (int k = lane; k < C * (kProbThreads / 32); k += 32) {
-            if (k % (kProbThreads / 32) >= T / 32) continue;
+        for (int k = lane; k < C * kProbWarps; k += 32) {
             const ProbPart p = first[k];
             if (p.m > m || (p.m == m && p.at < at)) { m = p.m; at = p.at; }
         }
         first_max(m, at);
-        for (int i = tid; i < n; i += T) out[i] = lo + i == at ? 1.0f : 0.0f;
+        for (int i = 0; i < left; i += T) out[i] = lo + tid + i == at ? 1.0f : 0.0f;
         return;
     }
 
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(kProbThreads, R <= 16 ? 3 : 2)
     for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) wm[w] = m;
     __syncthreads();
-    m = lane < T / 32 ? wm[lane] : -INFINITY;
+    m = lane < kProbWarps ? wm[lane] : -INFINITY;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     m = __shfl_sync(0xffffffffu, m, 0);
@@ -146,31 +149,37 @@ __global__ void __launch_bounds__(kProbThreads, R <= 16 ? 3 : 2)
     float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < R; k++) {
+        if (k % 4 == 0 && k * T >= n) break;  // none of the CTA's threads has more
         v[k] = exp_neg(v[k] - about, c);
         s += v[k];
     }
-    for (int i = tid + R * T; i < n; i += T) s += exp_neg(x[i] - about, c);
+    for (int i = R * T; i < left; i += T) s += exp_neg(x[i] - about, c);
     s = warp_sum(s);
     if (lane == 0) wsum[w] = s;
     __syncthreads();
     cluster_wait();
     if (w == 0) {
-        s = warp_sum(lane < T / 32 ? wsum[lane] : 0.0f);
+        s = warp_sum(lane < kProbWarps ? wsum[lane] : 0.0f);
         if (lane < C) *cl.map_shared_rank(&all[rank], lane) = ProbPart{m, s, 0, 0};
     }
     cluster_arrive();
     cluster_wait();
-    float M = -INFINITY, total = 0.0f;
-    for (int k = 0; k < C; k++) M = max_nan(M, all[k].m);
-    for (int k = 0; k < C; k++)
-        if (all[k].m > -INFINITY) total += all[k].s * exp_neg(all[k].m - M, c);
+    const ProbPart part = lane < C ? all[lane] : ProbPart{-INFINITY, 0.0f, 0, 0};
+    float M = part.m;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, o));
+    M = __shfl_sync(0xffffffffu, M, 0);
+    float total = part.m > -INFINITY ? part.s * exp_neg(part.m - M, c) : 0.0f;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total = __shfl_sync(0xffffffffu, total, 0);
     // 0 for a part (or a row) with nothing above -infinity; NaN where the row has a NaN or +infinity
     float f = m > -INFINITY ? __fdiv_rn(exp_neg(m - M, c), total) : 0.0f;
     if (!(M < INFINITY)) f = NAN;
 #pragma unroll
     for (int k = 0; k < R; k++)
-        if (tid + k * T < n) out[tid + k * T] = v[k] * f;
-    for (int i = tid + R * T; i < n; i += T) out[i] = exp_neg(x[i] - about, c) * f;
+        if (k * T < left) out[k * T] = v[k] * f;
+    for (int i = R * T; i < left; i += T) out[i] = exp_neg(x[i] - about, c) * f;
 }
 
 // ---------------------------------------------------------------------------
@@ -370,18 +379,16 @@ int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int 
     if (probs == logits && ld_logits != ld_probs) return GPT2B_ERR_INVALID_ARG;
     if (V > 1 << 30) return GPT2B_ERR_UNSUPPORTED;
     if (rows == 0) return GPT2B_OK;
-    // 16 entries a thread where 8 CTAs of 512 threads do with that; as many threads as that takes
+    // 16 entries a thread where 8 CTAs of 512 threads do with that
     const int cluster = row_cluster(V, 16 * kProbThreads);
     if ((long long)rows * cluster > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
     const ExpScale c = temperature == 0.0f ? ExpScale{0.0f, 0.0f, 0.0f} : exp_scale(temperature);
     const int share = (V + cluster - 1) / cluster, r = share <= 4 * kProbThreads ? 4 : share <= 16 * kProbThreads ? 16 : 32;
-    int threads = ((share + r - 1) / r + 31) / 32 * 32;
-    if (threads > kProbThreads) threads = kProbThreads;
     const cudaStream_t st = (cudaStream_t)stream;
     const long long li = ld_logits, lo = ld_probs;
-    if (r == 4) return status_from(launch_cluster(softmax_probs_kernel<4>, rows, cluster, threads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
-    if (r == 16) return status_from(launch_cluster(softmax_probs_kernel<16>, rows, cluster, threads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
-    return status_from(launch_cluster(softmax_probs_kernel<32>, rows, cluster, threads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
+    if (r == 4) return status_from(launch_cluster(softmax_probs_kernel<4>, rows, cluster, kProbThreads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
+    if (r == 16) return status_from(launch_cluster(softmax_probs_kernel<16>, rows, cluster, kProbThreads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
+    return status_from(launch_cluster(softmax_probs_kernel<32>, rows, cluster, kProbThreads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
 }
 
 int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* tokens, const float* target_probs,
