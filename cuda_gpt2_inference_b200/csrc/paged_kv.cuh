@@ -10,10 +10,16 @@ constexpr int kW4Group = 64;  // channels that share a step and a low end
 constexpr int kW4Tile = 16;   // block sizes are multiples of this, so a 16-row tile lies in one block
 constexpr int kTableMaxRequests = 4096;
 
-// (min, -max) of BF16 pairs; NaN wins, so one NaN in a group reaches its ends
+// of BF16 pairs; NaN wins, so one NaN in a group reaches its ends
 __device__ __forceinline__ uint32_t bf16x2_min_nan(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t bf16x2_max_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
@@ -24,10 +30,9 @@ __device__ __forceinline__ uint32_t bf16x2_min_nan(uint32_t a, uint32_t b) {
 // of range.  The step is rounded to nearest, not up: the top code then misses hi by at most 15 * 2^-8 of a
 // step, and no quotient reaches 15.5.  A group with a NaN or an infinity is held as NaN.
 //
-// Each code is the quotient rounded to the nearest whole number, ties to even.  A product with an approximate
-// reciprocal (off by 2^-20 of it at most) rounds to the same number unless it comes within 2^-16 of a half.
-// Where one of the eight does (BF16 values of one binade over a step of few bits tie often), each is put right
-// by its remainder d - code * step/2, which is exact: both products have at most 24 bits above d's last.
+// Each code is the quotient rounded to the nearest whole number, ties to even, where a quotient within 2^-17 of a
+// half counts as one.  The quotient is a product with an approximate reciprocal, off by 2^-19 at most, rounded to
+// a grid of 2^-16 on its way: a tie (frequent with BF16 values over a step of few bits) is one again there.
 __device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, float hi, uint32_t& meta) {
     const float c = 1.0f / 15.0f;
     if (!(fabsf(lo) < INFINITY && fabsf(hi) < INFINITY)) {
@@ -39,23 +44,14 @@ __device__ __forceinline__ uint32_t w4_encode8(const uint32_t* u, float lo, floa
     const uint32_t sbits = __bfloat16_as_ushort(__float2bfloat16_rn(t));
     meta = sbits | (__float_as_uint(lo) & 0xffff0000u);  // lo is a BF16 value
     if (sbits == 0) return 0u;
-    const float half = 0.5f * __uint_as_float(sbits << 16), nlo = -0.5f * lo, inv = __frcp_rn(half);
-    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-    float d[8], code[8], worst = 0.0f;
+    const float half = 0.5f * __uint_as_float(sbits << 16), nlo = -0.5f * lo, inv = __fdividef(1.0f, half);
+    constexpr float kGrid = 192.0f;        // added, it rounds 0 .. 15.5 to multiples of 2^-16
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: added, it rounds to a whole number
+    float code[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        d[k] = fmaf(k & 1 ? bf16hi(u[k / 2]) : bf16lo(u[k / 2]), 0.5f, nlo);  // the product is exact: one rounding
-        const float q = d[k] * inv;
-        code[k] = __fsub_rn(__fadd_rn(q, kRound), kRound);
-        worst = fmaxf(worst, fabsf(__fsub_rn(q, code[k])));
-    }
-    if (worst > 0.5f - 0x1p-16f) {
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float e = fmaf(-code[k], half, d[k]), twice = fabsf(e + e);
-            const bool odd = code[k] != 2.0f * rintf(0.5f * code[k]);
-            if (twice > half || (twice == half && odd)) code[k] += copysignf(1.0f, e);
-        }
+        const float d = fmaf(k & 1 ? bf16hi(u[k / 2]) : bf16lo(u[k / 2]), 0.5f, nlo);  // the product is exact
+        code[k] = __fsub_rn(__fadd_rn(fmaf(d, inv, kGrid), kRound - kGrid), kRound);
     }
     // four codes to a 16-bit whole number on the FMA units, its bits under the exponent of 2^23
     float h[2];

@@ -239,7 +239,8 @@ int gpt2b_attention_forward_kv_large_bf16_noalloc(uint16_t* out, const uint16_t*
  * Block tables are int32 [B][max_blocks]; entries behind a request's last block
  * are not read.  kv_cache, kv_scale, qkv and out are 16-byte aligned.
  * qkv rows are [Q (NH*hs) | K (NKV*hs) | V (NKV*hs)], ld elements apart.
- * A block (NKV * block_size * hs bytes of codes) is at most 2^31 - 1 bytes. */
+ * A block (NKV * block_size * hs bytes of codes) is at most 2^31 - 1 bytes, the codes
+ * of a layer's cache less than 2^37. */
 
 /* Block tables and row maps of one step, from the requests' lengths.  Request b
  * has ctx_lens[b] cached positions, new_lens[b] new rows (either may be 0;
@@ -267,7 +268,7 @@ int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions,
                           int block_size, int max_rows, int free_cap, gpt2b_stream_t stream);
 /* Appends rows' K and V at slot_map[row]: per group of 64 channels s =
  * bf16(max/15 - min/15) (0 below 2^-120), lo = min, code = round((x - lo)/s), ties
- * to even, at most 15.  A group with a NaN or an infinity is held as NaN.  A
+ * (quotients within 2^-17 of a half) to even, at most 15.  A group with a NaN or an infinity is held as NaN.  A
  * negative slot skips the row; a slot outside the cache is skipped and reported
  * (GPT2B_DEVERR_BAD_BLOCK).  The non-negative slots of a call must differ: of two
  * rows with one slot, either may be held, or a mix of their groups. */
