@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
     const int ratio = a.NH / a.NKV;
 
+    pdl_wait();
     pdl_trigger();  // the joining launch may wait on the SMs as they become free
     pa_scan(a, COLS, pre, wsum, blockIdx.x == 0);
     const long long total = pre[a.B];
@@ -809,7 +810,7 @@ template <int NG, int NT> static cudaError_t pa_launch(const PagedAttnArgs& a, c
     // one wave: no more CTAs than fit an SM's 228 KB of shared memory (1 KB of each is the system's)
     const int fit = (int)(228 * 1024 / (Sh::kSmem + pre + 1024 + 512));
     const int grid = sm_count() * (fit < Sh::kCtas ? fit : Sh::kCtas);
-    e = launch_k(paged_attn_kernel<NG, NT>, dim3(grid), dim3(kPaThreads), Sh::kSmem + pre, st, false, a);
+    e = launch_k(paged_attn_kernel<NG, NT>, dim3(grid), dim3(kPaThreads), Sh::kSmem + pre, st, true, a);
     if (e != cudaSuccess) return e;
     // a thread two channels of a column
     const unsigned parts = Sh::kCols * (Sh::kHS / 2) / kPaThreads;

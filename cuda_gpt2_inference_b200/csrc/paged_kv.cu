@@ -55,6 +55,7 @@ __global__ void __launch_bounds__(kTabThreads) block_tables_kernel(TableArgs a) 
     __shared__ long long w_rows[kTabThreads / 32], w_need[kTabThreads / 32];
     __shared__ int s_take;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    pdl_wait();
     const int F = min(max(*a.free_count, 0), a.free_cap);
     const long long most = (long long)a.max_blocks * a.block_size;
     if (tid == 0) s_take = 0;
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(kRwThreads)
                        int NH, int NKV, int hs, int ld, long long slots, int block_size, int parts, int rows_per_cta) {
     const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
     const RowPlace me = row_place(hs, block_size, per_row, part, parts, rows_per_cta);
+    pdl_wait();
     if (!me.active) return;  // per_row is a multiple of 16: the 16 lanes of a row leave together
     const uint32_t page = (uint32_t)(2 * NKV) * block_size * (hs / kW4Group);
     const long long step = (long long)(gridDim.x / parts) * rows_per_cta;
@@ -237,6 +239,7 @@ __global__ void __launch_bounds__(kRwThreads)
                       int NKV, int hs, long long slots, int block_size, int parts, int rows_per_cta) {
     const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
     const RowPlace me = row_place(hs, block_size, per_row, part, parts, rows_per_cta);
+    pdl_wait();
     if (!me.active) return;
     const uint32_t page = (uint32_t)(2 * NKV) * block_size * (hs / kW4Group);
     const long long step = (long long)(gridDim.x / parts) * rows_per_cta, ld = (long long)per_row * 8;
@@ -326,7 +329,7 @@ int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions,
     if (grid < 1) grid = 1;
     if (grid > sm_count()) grid = sm_count();
     return status_from(launch_k(block_tables_kernel, dim3((unsigned)grid), dim3(kTabThreads), 3 * sizeof(int) * (size_t)B,
-                                (cudaStream_t)stream, false, a));
+                                (cudaStream_t)stream, true, a));
 }
 
 static int w4_check(const void* codes, const void* scales, int NKV, int hs, int num_blocks, int block_size) {
@@ -352,7 +355,7 @@ int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_
     if (!aligned16(qkv) || ld % 8 != 0) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
     const RowGrid g = row_grid(rows, NKV, hs);
-    return status_from(launch_k(kv_write_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, false, kv_cache,
+    return status_from(launch_k(kv_write_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, true, kv_cache,
                                 (uint32_t*)kv_scale, (const __nv_bfloat16*)qkv, slot_map, rows, NH, NKV, hs, ld,
                                 (long long)num_blocks * block_size, block_size, g.parts, g.rows_per_cta));
 }
@@ -366,7 +369,7 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
     if (!aligned16(out)) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
     const RowGrid g = row_grid(rows, NKV, hs);
-    return status_from(launch_k(kv_read_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, false,
+    return status_from(launch_k(kv_read_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, true,
                                 (__nv_bfloat16*)out, kv_cache, (const uint32_t*)kv_scale, slot_map, rows, NKV, hs,
                                 (long long)num_blocks * block_size, block_size, g.parts, g.rows_per_cta));
 }

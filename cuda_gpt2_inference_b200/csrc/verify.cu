@@ -37,12 +37,14 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned rows, unsig
     cfg.gridDim = dim3(rows * cluster);
     cfg.blockDim = dim3(threads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
@@ -105,6 +107,7 @@ __global__ void __launch_bounds__(kProbThreads, R <= 16 ? 3 : 2)
 
     // entries in registers; -infinity behind the end.  NaN goes through the maximum.
     float v[R], m = -INFINITY;
+    pdl_wait();
     const int left = n - tid;  // entry k is there while k T < left
     x += tid;
     out += tid;
@@ -225,6 +228,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int b = blockIdx.x / C, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    pdl_wait();
     const int raw0 = a.row_start[b], raw1 = a.row_start[b + 1];
     const float u = a.u_sample[b];
     const int r0 = min(max(raw0, 0), a.rows), r1 = min(max(raw1, r0), a.rows);
