@@ -70,119 +70,120 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// One CTA of a row's cluster takes a contiguous part of it, R entries a thread in registers (entries beyond
-// 512 R are read twice more).  Each CTA sums e^((x - m)/T) about its own maximum m; the pairs (m, sum) are
-// exchanged behind the cluster's one barrier, and what a CTA holds about m is put right by one factor,
-// e^((m - M)/T) / total.  320 x 50257: 8 bytes an entry from and to HBM bound it; 5 rows: the chain launch - load
-// - exchange - store.
-constexpr int kProbThreads = 512, kProbWarps = kProbThreads / 32;
-
+// One CTA of a row's cluster takes a contiguous part of it.  A thread keeps a running maximum and a sum about it,
+// a warp joins its threads', and the pairs (m, sum) of all the cluster's warps are exchanged behind its one
+// barrier.  Then each thread reads its entries again, from L1 or L2 (unless one batch of loads was all), and writes
+// e^((x - M)/T) / total.  Nothing is kept in between, so 6 CTAs of 256 threads fit an SM and their loads, exchanges and stores overlap: 320 x 50257
+// takes 35 us, against 38 with the entries kept in registers (3 CTAs of 512 an SM) and 53 with those and the
+// next row's.  8 bytes an entry from and to HBM bound it (19.7 us).  Few rows: 512 threads with all loads in
+// flight at once; there the chain launch - load - exchange - store is what counts.
 struct ProbPart {
     float m, s;
-    int at, pad;
 };
-__device__ __forceinline__ void first_max(float& m, int& at) {
+
+template <int U, int T>
+__global__ void __launch_bounds__(T, T == 256 ? 6 : 2)
+    softmax_probs_kernel(float* probs, const float* logits, int V, long long ld_in, long long ld_out, ExpScale c) {
+    __shared__ ProbPart all[8 * (T / 32)];
+    cluster_begin();
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int share = (V + C - 1) / C, lo = min(rank * share, V);
+    const int left = min(share, V - lo) - (int)threadIdx.x;  // entry k is there while k T < left
+    const float* x = logits + (long long)(blockIdx.x / C) * ld_in + lo + threadIdx.x;
+    float* out = probs + (long long)(blockIdx.x / C) * ld_out + lo + threadIdx.x;
+
+    pdl_wait();
+    // NaN goes through the maximum.  In the sum a single product serves as exponent: its error grows with the
+    // distance from the maximum, but the terms fall faster (2^-22 of the sum at a spread of 10).
+    float v[U], m = -INFINITY, s = 0.0f;
+    for (int i = 0; i < left; i += U * T) {
+        float top = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+        for (int k = 0; k < U; k++) v[k] = i + k * T < left ? x[i + k * T] : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < U; k++) top = max_nan(top, v[k]);
+        const float about = top > -INFINITY ? top : 0.0f;
+        s *= exp2f((m - about) * c.hi);
+#pragma unroll
+        for (int k = 0; k < U; k++) s += exp2f((v[k] - about) * c.hi);
+        m = top;
+    }
+    float M = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, o));
+    s = warp_sum(m > -INFINITY ? s * exp_neg(m - M, c) : 0.0f);
+    cluster_wait();
+    if (lane < C) *cl.map_shared_rank(&all[rank * (T / 32) + w], lane) = ProbPart{M, s};
+    cluster_arrive();
+    cluster_wait();
+    M = -INFINITY;
+    for (int k = lane; k < C * (T / 32); k += 32) M = max_nan(M, all[k].m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, o));
+    s = 0.0f;
+    for (int k = lane; k < C * (T / 32); k += 32)
+        if (all[k].m > -INFINITY) s += all[k].s * exp_neg(all[k].m - M, c);
+    s = warp_sum(s);
+    // zeros where the row has nothing above -infinity, NaN where it has a NaN or +infinity
+    float inv = M > -INFINITY ? __frcp_rn(s) : 0.0f;
+    if (!(M < INFINITY)) inv = NAN;
+    const float about = M > -INFINITY ? M : 0.0f;
+    for (int i = 0; i < left; i += U * T) {
+        if (share > U * T) {
+#pragma unroll
+            for (int k = 0; k < U; k++)
+                if (i + k * T < left) v[k] = x[i + k * T];
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++)
+            if (i + k * T < left) out[i + k * T] = exp_neg(v[k] - about, c) * inv;
     }
 }
 
-template <int R>
-__global__ void __launch_bounds__(kProbThreads, R <= 16 ? 3 : 2)
-    softmax_probs_kernel(float* probs, const float* logits, int V, long long ld_in, long long ld_out, bool greedy, ExpScale c) {
-    __shared__ float wm[kProbWarps], wsum[kProbWarps];
-    __shared__ ProbPart all[8];
+// Temperature 0: 1 at the first largest, NaN left out.
+struct FirstMax {
+    float m;
+    int at;
+};
+__device__ __forceinline__ FirstMax first_max(FirstMax a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, a.m, o);
+        const int at = __shfl_xor_sync(0xffffffffu, a.at, o);
+        if (m > a.m || (m == a.m && at < a.at)) a = {m, at};
+    }
+    return a;
+}
+constexpr int kProbThreads = 512, kProbWarps = kProbThreads / 32;
+
+__global__ void __launch_bounds__(kProbThreads)
+    greedy_probs_kernel(float* probs, const float* logits, int V, long long ld_in, long long ld_out) {
+    __shared__ FirstMax all[8 * kProbWarps];
     cluster_begin();
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    constexpr int T = kProbThreads;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    const long long row = blockIdx.x / C;
-    const int share = (V + C - 1) / C, lo = min(rank * share, V), n = min(share, V - lo);
-    const float* x = logits + row * ld_in + lo;
-    float* out = probs + row * ld_out + lo;
-
-    // entries in registers; -infinity behind the end.  NaN goes through the maximum.
-    float v[R], m = -INFINITY;
+    const int share = (V + C - 1) / C, lo = min(rank * share, V), hi = min(lo + share, V);
+    const float* x = logits + (long long)(blockIdx.x / C) * ld_in;
+    float* out = probs + (long long)(blockIdx.x / C) * ld_out;
     pdl_wait();
-    const int left = n - tid;  // entry k is there while k T < left
-    x += tid;
-    out += tid;
-#pragma unroll
-    for (int k = 0; k < R; k++) v[k] = k * T < left ? x[k * T] : -INFINITY;
-#pragma unroll
-    for (int k = 0; k < R; k++) m = max_nan(m, v[k]);
-    for (int i = R * T; i < left; i += T) m = max_nan(m, x[i]);
-
-    if (greedy) {  // the first largest, NaN left out
-        m = -INFINITY;
-        int at = INT_MAX;
-        for (int i = 0; i < left; i += T)
-            if (x[i] > m) { m = x[i]; at = lo + tid + i; }
-        first_max(m, at);
-        cluster_wait();
-        __shared__ ProbPart first[8 * kProbWarps];
-        if (lane < C) *cl.map_shared_rank(&first[rank * kProbWarps + w], lane) = ProbPart{m, 0.0f, at, 0};
-        cluster_arrive();
-        cluster_wait();
-        m = -INFINITY;
-        at = INT_MAX;
-        for (int k = lane; k < C * kProbWarps; k += 32) {
-            const ProbPart p = first[k];
-            if (p.m > m || (p.m == m && p.at < at)) { m = p.m; at = p.at; }
-        }
-        first_max(m, at);
-        for (int i = 0; i < left; i += T) out[i] = lo + tid + i == at ? 1.0f : 0.0f;
-        return;
+    FirstMax a{-INFINITY, INT_MAX};
+#pragma unroll 8
+    for (int i = lo + tid; i < hi; i += kProbThreads) {
+        const float y = x[i];
+        if (y > a.m) a = {y, i};
     }
-
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) wm[w] = m;
-    __syncthreads();
-    m = lane < kProbWarps ? wm[lane] : -INFINITY;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    m = __shfl_sync(0xffffffffu, m, 0);
-    // about m; a part with nothing above -infinity holds zeros
-    const float about = m > -INFINITY ? m : 0.0f;
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < R; k++) {
-        if (k % 4 == 0 && k * T >= n) break;  // none of the CTA's threads has more
-        v[k] = exp_neg(v[k] - about, c);
-        s += v[k];
-    }
-    for (int i = R * T; i < left; i += T) s += exp_neg(x[i] - about, c);
-    s = warp_sum(s);
-    if (lane == 0) wsum[w] = s;
-    __syncthreads();
+    a = first_max(a);
     cluster_wait();
-    if (w == 0) {
-        s = warp_sum(lane < kProbWarps ? wsum[lane] : 0.0f);
-        if (lane < C) *cl.map_shared_rank(&all[rank], lane) = ProbPart{m, s, 0, 0};
-    }
+    if (lane < C) *cl.map_shared_rank(&all[rank * kProbWarps + w], lane) = a;
     cluster_arrive();
     cluster_wait();
-    const ProbPart part = lane < C ? all[lane] : ProbPart{-INFINITY, 0.0f, 0, 0};
-    float M = part.m;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, o));
-    M = __shfl_sync(0xffffffffu, M, 0);
-    float total = part.m > -INFINITY ? part.s * exp_neg(part.m - M, c) : 0.0f;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total = __shfl_sync(0xffffffffu, total, 0);
-    // 0 for a part (or a row) with nothing above -infinity; NaN where the row has a NaN or +infinity
-    float f = m > -INFINITY ? __fdiv_rn(exp_neg(m - M, c), total) : 0.0f;
-    if (!(M < INFINITY)) f = NAN;
-#pragma unroll
-    for (int k = 0; k < R; k++)
-        if (k * T < left) out[k * T] = v[k] * f;
-    for (int i = R * T; i < left; i += T) out[i] = exp_neg(x[i] - about, c) * f;
+    a = {-INFINITY, INT_MAX};
+    for (int k = lane; k < C * kProbWarps; k += 32)
+        if (all[k].m > a.m || (all[k].m == a.m && all[k].at < a.at)) a = all[k];
+    a = first_max(a);
+    for (int i = lo + tid; i < hi; i += kProbThreads) out[i] = i == a.at ? 1.0f : 0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -351,18 +352,25 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
         const unsigned some = __ballot_sync(0xffffffffu, sum > 0.0);
         const int src = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
         if (src >= 0) {
-            double at = run + before;
-            int mine = -1, last = -1;
-            if (lane == src) {
-                for (int k = from; k < to && mine < 0; k++) {
-                    const double v = wt(k);
-                    at += v;
-                    if (v > 0.0) last = k;
-                    if (at > t && (v > 0.0 || t < 0.0)) mine = k;
+            // that run's entries, a lane each
+            run += __shfl_sync(0xffffffffu, before, src);
+            const int begin = __shfl_sync(0xffffffffu, from, src), stop = __shfl_sync(0xffffffffu, to, src);
+            int found = -1, last = -1;
+            for (int k0 = begin; k0 < stop && found < 0; k0 += 32) {
+                const double v = k0 + lane < stop ? wt(k0 + lane) : 0.0;
+                double sofar = v;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double up = __shfl_up_sync(0xffffffffu, sofar, o);
+                    if (lane >= o) sofar += up;
                 }
-                if (mine < 0) mine = last;
+                const unsigned hit = __ballot_sync(0xffffffffu, run + sofar > t && (v > 0.0 || t < 0.0));
+                const unsigned any = __ballot_sync(0xffffffffu, v > 0.0);
+                if (hit) found = k0 + __ffs(hit) - 1;
+                if (any) last = k0 + 31 - __clz(any);
+                run += __shfl_sync(0xffffffffu, sofar, 31);
             }
-            pick = __shfl_sync(0xffffffffu, mine, src);
+            pick = found >= 0 ? found : last;
         }
     }
     for (int i = lane; i < a.max_out; i += 32) out[i] = i < taken ? a.tokens[r0 + 1 + i] : i == taken ? pick : -1;
@@ -383,16 +391,16 @@ int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int 
     if (probs == logits && ld_logits != ld_probs) return GPT2B_ERR_INVALID_ARG;
     if (V > 1 << 30) return GPT2B_ERR_UNSUPPORTED;
     if (rows == 0) return GPT2B_OK;
-    // 16 entries a thread where 8 CTAs of 512 threads do with that
     const int cluster = row_cluster(V, 16 * kProbThreads);
     if ((long long)rows * cluster > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
-    const ExpScale c = temperature == 0.0f ? ExpScale{0.0f, 0.0f, 0.0f} : exp_scale(temperature);
-    const int share = (V + cluster - 1) / cluster, r = share <= 4 * kProbThreads ? 4 : share <= 16 * kProbThreads ? 16 : 32;
     const cudaStream_t st = (cudaStream_t)stream;
     const long long li = ld_logits, lo = ld_probs;
-    if (r == 4) return status_from(launch_cluster(softmax_probs_kernel<4>, rows, cluster, kProbThreads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
-    if (r == 16) return status_from(launch_cluster(softmax_probs_kernel<16>, rows, cluster, kProbThreads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
-    return status_from(launch_cluster(softmax_probs_kernel<32>, rows, cluster, kProbThreads, st, probs, logits, V, li, lo, temperature == 0.0f, c));
+    if (temperature == 0.0f)
+        return status_from(launch_cluster(greedy_probs_kernel, rows, cluster, kProbThreads, st, probs, logits, V, li, lo));
+    const ExpScale c = exp_scale(temperature);
+    if ((long long)rows * cluster <= 2ll * sm_count())
+        return status_from(launch_cluster(softmax_probs_kernel<16, 512>, rows, cluster, 512, st, probs, logits, V, li, lo, c));
+    return status_from(launch_cluster(softmax_probs_kernel<16, 256>, rows, cluster, 256, st, probs, logits, V, li, lo, c));
 }
 
 int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* tokens, const float* target_probs,
