@@ -63,8 +63,7 @@ def test_append_holds_the_defined_codes(cuda, gpt2b, NKV, ratio, hs, bs, rows, k
     # the step of subnormal-range groups may differ where the products underflow; there the values are compared below
     got_c, got_s = dc.cpu(), ds.cpu()
     assert torch.equal(got_s.view(torch.int16), scales.view(torch.int16)) or kind == "small"
-    # the quotient is rounded once in 32 bits and once to a whole number: codes differ from the 64-bit
-    # form's only where that lands on the other side of a tie, by one
+    # quotients within 2^-17 of a half count as one: codes differ from the 64-bit form's only there, by one
     diff = torch.stack([got_c & 15, got_c >> 4]).int() - torch.stack([codes & 15, codes >> 4]).int()
     assert diff.abs().max() <= 1
     assert (diff != 0).float().mean() < 1e-3
@@ -427,3 +426,96 @@ def test_operators_on_the_tensors_own_device(cuda):
         d = [t.to("cuda:0") for t in st[1:]]
         ops.attention_forward_paged_w4(out, *d[:3], *d[3:], 2, 1, ws)
     _check_attention(st, out)
+
+
+# ------------------------------------------------------------------- ordering ----
+def test_calls_wait_for_whatever_came_before(cuda):
+    """The kernels are launched before their predecessor has ended; copies, fills, kernels of other libraries and
+    joins of streams in front of them are waited for all the same, eagerly and captured."""
+    from cuda_gpt2_inference_b200 import ops
+    NKV, NH, hs, bs, nb, n = 4, 8, 128, 16, 600, 4096
+    g = torch.Generator().manual_seed(21)
+    qkv = torch.randn(n, (NH + 2 * NKV) * hs, generator=g).to(BF).cuda()
+    slots = torch.randperm(nb * bs, generator=g)[:n].cuda()
+    src = torch.zeros_like(qkv)
+    codes = torch.zeros(nb, 2, NKV, bs, hs // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(nb, 2, NKV, bs, hs // 64, 2, dtype=BF, device="cuda")
+    out, copy = torch.zeros(n, 2, NKV, hs, dtype=BF, device="cuda"), torch.zeros(n, 2, NKV, hs, dtype=BF, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        codes.zero_(), scales.zero_(), out.zero_()      # fills
+        src.copy_(qkv)                                   # a copy right in front of the append
+        ops.kv_cache_write_w4(codes, scales, src, slots, NH)
+        src.zero_()                                      # and a fill of what it reads right behind it
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            torch.mm(big, big)                           # some time on another stream
+            ops.kv_cache_read_w4(out, codes, scales, slots)
+        here.wait_stream(side)
+        ops.kv_cache_write_w4(codes, scales, src, slots, NH)   # overwrites behind the join
+        copy.copy_(out)
+        ops.kv_cache_read_w4(out, codes, scales, slots)
+
+    kv = qkv[:, NH * hs:].view(n, 2, NKV, hs).cpu()
+    c, s = plain.quantise(kv)
+    want = plain.values(c, s)
+    tol = plain.BF16 * want.abs() + s[..., 0].double().repeat_interleave(64, -1) * 1e-2  # (ties: see the append's test)
+
+    def check():
+        torch.cuda.synchronize()
+        near = (copy.cpu().double() - want).abs() <= tol
+        assert near.float().mean() > 0.999
+        assert ((copy.cpu().double() - want).abs() <= tol + s[..., 0].double().repeat_interleave(64, -1)).all()
+        assert not out.any()
+
+    run()
+    check()
+    work = torch.cuda.Stream()
+    work.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(work), torch.cuda.graph(graph, stream=work):
+        run()
+    for _ in range(3):
+        copy.zero_()
+        graph.replay()
+        check()
+
+
+def test_attention_hides_what_a_row_does_not_see(cuda):
+    """A draft's own position may hold NaN (a group with an infinity): the rows before it do not see it."""
+    for NKV, ratio, hs in ((2, 1, 64), (1, 8, 128), (2, 4, 64)):
+        NH, qkv, codes, scales, table, lens, start = _attention_state(NKV, ratio, hs, 16, [70, 45], [5, 3], 31)
+        for b, n in ((0, 70), (1, 45)):
+            scales[int(table[b, (n - 1) // 16]), :, :, (n - 1) % 16] = math.nan
+        out = _attend((NH, qkv, codes, scales, table, lens, start), 5).cpu()
+        rows = [0, 1, 2, 3, 5, 6]
+        assert out[[4, 7]].isnan().all()
+        clean = scales.clone()
+        for b, n in ((0, 70), (1, 45)):
+            clean[int(table[b, (n - 1) // 16]), :, :, (n - 1) % 16] = 0
+        want, err = plain.attention(qkv, codes, clean, table, lens, start, NH)
+        off = (out[rows].double() - want[rows]).abs()
+        assert (off <= plain.BF16 * want[rows].abs() + (1 + plain.BF16) * err[rows] + 2.0 ** -126).all()
+
+
+def test_attention_of_two_calls_at_once(cuda):
+    """Two streams with a workspace each, and the same call again and again on one."""
+    from cuda_gpt2_inference_b200 import ops
+    sts = [_attention_state(2, 2, 64, 16, [900, 33, 400], [2, 1, 3], 40 + k) for k in range(2)]
+    want = [_attend(st, 3) for st in sts]
+    ds = [[t.cuda() for t in st[1:]] for st in sts]
+    ws = [torch.empty(ops.attention_paged_w4_workspace(4, 2, 64, 3), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[torch.full_like(want[k], 123.0) for _ in range(20)] for k in range(2)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for k in range(2):
+            d = ds[k]
+            ops.attention_forward_paged_w4(outs[k][i], d[0], d[1], d[2], d[3], d[4], d[5], 4, 3, ws[k], stream=streams[k])
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(o, want[k]) for o in outs[k])
