@@ -225,7 +225,10 @@ constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // nibbles as code 
 // the 4 even or odd rows of a V load (4 bytes a lane) each fall in distinct banks.
 __device__ __forceinline__ int tile_pos(int r) { return r ^ ((r >> 2) & 1); }
 
-template <int NG, int NT>
+// PAIR: the block size is a multiple of 32, so a step's two tiles lie in one block, one behind the other.  That
+// leaves one block to look up and one address to work out a step: 32 x 8192 positions of 25 heads of 64 take 106
+// us against 113, 32 x 16384 of 8 heads of 128 with 16 columns 169 against 177.
+template <int NG, int NT, bool PAIR>
 __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn_kernel(PagedAttnArgs a) {
     using Sh = PaShape<NG, NT>;
     constexpr int HS = Sh::kHS, COLS = Sh::kCols, STAGES = Sh::kStages;
@@ -302,11 +305,13 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         auto fetch = [&]() {
             Step f{0, 0, 0, 0};
             if (f_pos < p_end) {
-                const bool next = f_off + 16 >= a.block_size, two = f_pos + 16 < p_end;
                 f.off0 = f_off;
-                f.off1 = two ? (next ? 0 : f_off + 16) : f_off;  // behind the end: the first tile again
-                f.blk0 = table[f_idx];
-                f.blk1 = table[f_idx + (two && next)];
+                f.blk0 = f.blk1 = table[f_idx];
+                if constexpr (!PAIR) {
+                    const bool next = f_off + 16 >= a.block_size, two = f_pos + 16 < p_end;
+                    f.off1 = two ? (next ? 0 : f_off + 16) : f_off;  // behind the end: the first tile again
+                    f.blk1 = table[f_idx + (two && next)];
+                }
                 f_pos += kPaUnit;
                 f_idx += a.unit_blocks;
                 f_off += a.unit_rest;
@@ -320,7 +325,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
         auto issue = [&](Step f, int it, int stage) {
             if (it < steps) {
                 const uint32_t base = ring + stage * Sh::kStageBytes;
-                const bool bad0 = (unsigned)f.blk0 >= (unsigned)a.num_blocks, bad1 = (unsigned)f.blk1 >= (unsigned)a.num_blocks;
+                const bool bad0 = (unsigned)f.blk0 >= (unsigned)a.num_blocks;
+                const bool bad1 = PAIR ? bad0 : (unsigned)f.blk1 >= (unsigned)a.num_blocks;
                 bad &= ~(3u << (2 * stage));
                 if (bad0 || bad1) {  // left out: block 0 is read in its place and masked
                     bad |= (bad0 ? 1u : 0u) << (2 * stage) | (bad1 ? 2u : 0u) << (2 * stage);
@@ -328,8 +334,9 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     if (bad1) f.blk1 = 0;
                     if (lane == 0) report_device_error(GPT2B_DEVERR_BAD_BLOCK);
                 }
-                const uint8_t* src[2] = {k_src + ((size_t)(uint32_t)f.blk0 * page + (uint32_t)f.off0 * (HS / 2)),
-                                         k_src + ((size_t)(uint32_t)f.blk1 * page + (uint32_t)f.off1 * (HS / 2))};
+                const uint8_t* src0 = k_src + ((size_t)(uint32_t)f.blk0 * page + (uint32_t)f.off0 * (HS / 2));
+                const uint8_t* src[2] = {src0, PAIR ? src0 + 16 * (HS / 2)
+                                                    : k_src + ((size_t)(uint32_t)f.blk1 * page + (uint32_t)f.off1 * (HS / 2))};
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -342,7 +349,9 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 const bool hi = lane >= 8 * NG;
                 if (lane < 16 * NG)
                     cp_async16(base + 2 * Sh::kCodeBytes + (v_meta ? Sh::kMetaBytes : 0) + (hi ? 64 * NG : 0) + lane % (4 * NG) * 16,
-                               m_src + ((size_t)(uint32_t)(hi ? f.blk1 : f.blk0) * meta_page + (uint32_t)(hi ? f.off1 : f.off0) * (4 * NG)));
+                               PAIR ? m_src + (hi ? 64 * NG : 0) + ((size_t)(uint32_t)f.blk0 * meta_page + (uint32_t)f.off0 * (4 * NG))
+                                    : m_src + ((size_t)(uint32_t)(hi ? f.blk1 : f.blk0) * meta_page +
+                                               (uint32_t)(hi ? f.off1 : f.off0) * (4 * NG)));
             }
             cp_async_commit();
         };
@@ -800,21 +809,25 @@ template <int NG, int NT> static size_t pa_workspace() {
     return (size_t)sm_count() * PaShape<NG, NT>::kCtas * 2 * PaShape<NG, NT>::kSlot * sizeof(float);
 }
 
-template <int NG, int NT> static cudaError_t pa_launch(const PagedAttnArgs& a, cudaStream_t st) {
+template <int NG, int NT, bool PAIR> static cudaError_t pa_launch(const PagedAttnArgs& a, cudaStream_t st) {
     using Sh = PaShape<NG, NT>;
     static unsigned long long mask = 0, mask2 = 0;
-    cudaError_t e = ensure_smem_limit(paged_attn_kernel<NG, NT>, &mask);
+    cudaError_t e = ensure_smem_limit(paged_attn_kernel<NG, NT, PAIR>, &mask);
     if (e == cudaSuccess) e = ensure_smem_limit(paged_attn_join_kernel<NG, NT>, &mask2);
     if (e != cudaSuccess) return e;
     const size_t pre = sizeof(long long) * ((size_t)a.B + 1);
     // one wave: no more CTAs than fit an SM's 228 KB of shared memory (1 KB of each is the system's)
     const int fit = (int)(228 * 1024 / (Sh::kSmem + pre + 1024 + 512));
     const int grid = sm_count() * (fit < Sh::kCtas ? fit : Sh::kCtas);
-    e = launch_k(paged_attn_kernel<NG, NT>, dim3(grid), dim3(kPaThreads), Sh::kSmem + pre, st, true, a);
+    e = launch_k(paged_attn_kernel<NG, NT, PAIR>, dim3(grid), dim3(kPaThreads), Sh::kSmem + pre, st, true, a);
     if (e != cudaSuccess) return e;
     // a thread two channels of a column
     const unsigned parts = Sh::kCols * (Sh::kHS / 2) / kPaThreads;
     return launch_k(paged_attn_join_kernel<NG, NT>, dim3(grid - 1, parts), dim3(kPaThreads), pre, st, true, a, grid);
+}
+
+template <int NG, int NT> static cudaError_t pa_launch(const PagedAttnArgs& a, cudaStream_t st) {
+    return a.block_size % kPaStep == 0 ? pa_launch<NG, NT, true>(a, st) : pa_launch<NG, NT, false>(a, st);
 }
 
 }  // namespace gpt2b
