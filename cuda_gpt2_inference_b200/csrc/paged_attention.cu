@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 
 // Joins the pieces of the segments that several CTAs shared: block i takes the segment that the border between
 // the runs of CTAs i and i + 1 cuts, if that is the segment's first border.  A thread holds two channels of a
-// column, a warp one column; pieces are added in the order of their CTAs.  Launched early: its CTAs find their
+// column; pieces are added in the order of their CTAs.  Launched early: its CTAs find their
 // segments while the last of the main ones still run.
 template <int NG, int NT>
 __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnArgs a, int main_grid) {
@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
     pa_scan(a, COLS, pre, wsum, false);
     const long long total = pre[a.B], G = min((long long)main_grid, total);
     const long long i0 = blockIdx.x;
-    const int ratio = a.NH / a.NKV, lane = threadIdx.x & 31;
+    const int ratio = a.NH / a.NKV;
     bool mine = false;
     int b = 0, kvh = 0, chunk = 0, pieces = 0;
     PaRequest rq{};
@@ -772,30 +772,43 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
     const int col = i / (HS / 2), ch = 2 * (i % (HS / 2));
     mine = mine && col < min(COLS, rq.n * ratio - chunk * COLS);
     pdl_wait();
-    if (!mine) return;  // whole warps
+    if (!mine) return;
     // piece k > 0 is slot 0 of CTA i0 + k, the first slot 1 of CTA i0
     const float* first = a.ws + ((size_t)i0 * 2 + 1) * Sh::kSlot;
     auto slot = [&](int k) { return k == 0 ? first : first + (2 * (size_t)k - 1) * Sh::kSlot; };
+    constexpr int kAhead = 16;  // pieces whose results are on their way together
     float M = -FLT_MAX, x = 0.0f, y = 0.0f, sum = 0.0f;
-    for (int k = lane; k < pieces; k += 32) M = fmaxf(M, slot(k)[COLS * HS + col]);
-    M = warp_max(M);
-    for (int k0 = 0; k0 < pieces; k0 += 32) {
-        float f = 0.0f;
-        if (k0 + lane < pieces) {
-            const float* s = slot(k0 + lane);
-            f = ex2(s[COLS * HS + col] - M);
-            sum = fmaf(s[COLS * HS + COLS + col], f, sum);
+    for (int k0 = 0; k0 < pieces; k0 += kAhead) {
+        float m[kAhead], l[kAhead];
+        float2 o[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            m[k] = -FLT_MAX;
+            l[k] = 0.0f;
+            o[k] = make_float2(0.0f, 0.0f);
+            if (k0 + k < pieces) {
+                const float* s = slot(k0 + k);
+                m[k] = s[COLS * HS + col];
+                l[k] = s[COLS * HS + COLS + col];
+                o[k] = *reinterpret_cast<const float2*>(s + col * HS + ch);
+            }
         }
-        const int n = min(32, pieces - k0);
-#pragma unroll 8
-        for (int k = 0; k < n; k++) {
-            const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float2 o = *reinterpret_cast<const float2*>(slot(k0 + k) + col * HS + ch);
-            x = fmaf(o.x, fk, x);
-            y = fmaf(o.y, fk, y);
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) top = fmaxf(top, m[k]);
+        const float f = ex2(M - top);
+        x *= f;
+        y *= f;
+        sum *= f;
+        M = top;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const float fk = ex2(m[k] - M);
+            x = fmaf(o[k].x, fk, x);
+            y = fmaf(o[k].y, fk, y);
+            sum = fmaf(l[k], fk, sum);
         }
     }
-    sum = warp_sum(sum);
     const int gc = chunk * COLS + col;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     __nv_bfloat16* o = a.out + (size_t)(rq.r0 + gc / ratio) * a.NH * HS + (size_t)(kvh * ratio + gc % ratio) * HS + ch;

@@ -151,12 +151,13 @@ __global__ void __launch_bounds__(kTabThreads) block_tables_kernel(TableArgs a) 
 // ---------------------------------------------------------------------------
 // append and read-back
 // ---------------------------------------------------------------------------
-// A thread holds 8 channels (one 16-byte access of BF16, one 4-byte access of codes), 8 threads a group of 64.
-// A CTA's threads cover whole rows, so a thread's head and channels are worked out once.  The 16 lanes that
-// share a row work out the places of their next 16 rows together, one each, and hand them round as numbers of
-// 32-byte groups of codes (a step to each, in the same order).  kRowsAhead rows' loads are in flight: 4 took 55 us
-// for 16384 rows of 2 * 8 * 128 appended and read back, 2 58, 8 70.
-constexpr int kRwThreads = 256, kRowsAhead = 4;
+// Appending, a thread holds 16 channels (two 16-byte loads of BF16, one 8-byte store of codes), 4 threads a group
+// of 64; reading back 8 (one 4-byte load of codes, one 16-byte store: with 32 bytes a thread the stores of a warp
+// left gaps, 24 us against 19).  A CTA's threads cover whole rows, so a thread's head and channels are worked out
+// once.  The 8 lanes that share a row (at least) work out the places of their next 8 rows together, one each, and
+// hand them round as numbers of 32-byte groups of codes (a step to each, in the same order).  Several rows' loads
+// are in flight.  16384 rows of 2 * 8 * 128: 22 us to append and 19 to read back, of 13 each that HBM takes.
+constexpr int kRwThreads = 256, kWriteChannels = 16, kReadChannels = 8, kWriteAhead = 2, kReadAhead = 4;
 constexpr uint32_t kNoRow = 0xffffffffu;
 
 struct RowPlace {
@@ -164,11 +165,11 @@ struct RowPlace {
     uint32_t group;  // this thread's group of codes in a block, at offset 0
     bool active;
 };
-__device__ __forceinline__ RowPlace row_place(int hs, int block_size, int per_row, int part, int parts, int rows_per_cta) {
+__device__ __forceinline__ RowPlace row_place(int channels, int hs, int block_size, int per_row, int part, int parts, int rows_per_cta) {
     RowPlace r;
     const int i = part * kRwThreads + threadIdx.x;  // thread of the row pass, over all parts of a wide row
     r.row = parts > 1 ? 0 : i / per_row;
-    r.col = (i - r.row * per_row) * 8;
+    r.col = (i - r.row * per_row) * channels;
     r.active = parts > 1 ? i < per_row : r.row < rows_per_cta;
     const int head = r.col / hs, d = r.col - head * hs;  // head of [K | V]
     r.group = (uint32_t)head * block_size * (hs / kW4Group) + d / kW4Group;
@@ -189,45 +190,53 @@ __device__ __forceinline__ uint32_t slot_group(long long slot, long long slots, 
 __global__ void __launch_bounds__(kRwThreads)
     kv_write_w4_kernel(uint8_t* codes, uint32_t* scales, const __nv_bfloat16* qkv, const long long* slot_map, int rows,
                        int NH, int NKV, int hs, int ld, long long slots, int block_size, int parts, int rows_per_cta) {
-    const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
-    const RowPlace me = row_place(hs, block_size, per_row, part, parts, rows_per_cta);
+    const int per_row = 2 * NKV * hs / kWriteChannels, part = blockIdx.x % parts;
+    const RowPlace me = row_place(kWriteChannels, hs, block_size, per_row, part, parts, rows_per_cta);
     pdl_wait();
-    if (!me.active) return;  // per_row is a multiple of 16: the 16 lanes of a row leave together
+    if (!me.active) return;  // per_row is a multiple of 8: the 8 lanes of a row leave together
     const uint32_t page = (uint32_t)(2 * NKV) * block_size * (hs / kW4Group);
     const long long step = (long long)(gridDim.x / parts) * rows_per_cta;
     const __nv_bfloat16* src = qkv + (size_t)NH * hs + me.col;
     uint8_t* my_codes = codes + (size_t)me.group * (kW4Group / 2) + (me.col & (kW4Group - 1)) / 2;
     uint32_t* my_scales = scales + me.group;
-    const unsigned sixteen = 0xffffu << (threadIdx.x & 16);
+    const unsigned eight = 0xffu << (threadIdx.x & 24);
     const bool first = (me.col & (kW4Group - 1)) == 0;
-    for (long long base = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; base < rows; base += 16 * step) {
-        const long long ahead = base + (threadIdx.x & 15) * step;
+    for (long long base = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; base < rows; base += 8 * step) {
+        const long long ahead = base + (threadIdx.x & 7) * step;
         const uint32_t place =
             ahead < rows ? slot_group(slot_map[ahead], slots, block_size, hs / kW4Group, page) : kNoRow;
         const __nv_bfloat16* row = src + base * ld;
-        const int n = (int)min(16ll, (rows - base + step - 1) / step);
-        for (int k0 = 0; k0 < n; k0 += kRowsAhead) {
-            uint4 v[kRowsAhead];
-            uint32_t at[kRowsAhead];
+        const int n = (int)min(8ll, (rows - base + step - 1) / step);
+        for (int k0 = 0; k0 < n; k0 += kWriteAhead) {
+            uint4 v[kWriteAhead][2];
+            uint32_t at[kWriteAhead];
 #pragma unroll
-            for (int k = 0; k < kRowsAhead; k++) {
-                at[k] = __shfl_sync(sixteen, place, k0 + k, 16);
-                if (at[k] != kNoRow) v[k] = *reinterpret_cast<const uint4*>(row);
+            for (int k = 0; k < kWriteAhead; k++) {
+                at[k] = __shfl_sync(eight, place, k0 + k, 8);
+                if (at[k] != kNoRow) {
+                    v[k][0] = reinterpret_cast<const uint4*>(row)[0];
+                    v[k][1] = reinterpret_cast<const uint4*>(row)[1];
+                }
                 row += step * ld;
             }
 #pragma unroll
-            for (int k = 0; k < kRowsAhead; k++) {
+            for (int k = 0; k < kWriteAhead; k++) {
                 if (at[k] == kNoRow) continue;
-                const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-                // ends of the group as (min, -max): pairs, then the two halves, then 8 threads
-                uint32_t mn = bf16x2_min_nan(bf16x2_min_nan(u[0], u[1]), bf16x2_min_nan(u[2], u[3]));
-                uint32_t mx = bf16x2_max_nan(bf16x2_max_nan(u[0], u[1]), bf16x2_max_nan(u[2], u[3])) ^ 0x80008000u;
+                const uint32_t u[8] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w, v[k][1].x, v[k][1].y, v[k][1].z, v[k][1].w};
+                // ends of the group as (min, -max): pairs, then the two halves, then 4 threads
+                uint32_t mn = u[0], mx = u[0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) {
+                    mn = bf16x2_min_nan(mn, u[i]);
+                    mx = bf16x2_max_nan(mx, u[i]);
+                }
+                mx ^= 0x80008000u;
                 uint32_t e = bf16x2_min_nan(__byte_perm(mn, mx, 0x5410), __byte_perm(mn, mx, 0x7632));
 #pragma unroll
-                for (int o = 4; o > 0; o >>= 1) e = bf16x2_min_nan(e, __shfl_xor_sync(sixteen, e, o));
+                for (int o = 2; o > 0; o >>= 1) e = bf16x2_min_nan(e, __shfl_xor_sync(eight, e, o));
                 uint32_t meta;
-                const uint32_t word = w4_encode8(u, bf16lo(e), -bf16hi(e), meta);
-                *reinterpret_cast<uint32_t*>(my_codes + (size_t)at[k] * (kW4Group / 2)) = word;
+                *reinterpret_cast<uint2*>(my_codes + (size_t)at[k] * (kW4Group / 2)) =
+                    w4_encode16(u, bf16lo(e), -bf16hi(e), meta);
                 if (first) my_scales[at[k]] = meta;
             }
         }
@@ -237,26 +246,26 @@ __global__ void __launch_bounds__(kRwThreads)
 __global__ void __launch_bounds__(kRwThreads)
     kv_read_w4_kernel(__nv_bfloat16* out, const uint8_t* codes, const uint32_t* scales, const long long* slot_map, int rows,
                       int NKV, int hs, long long slots, int block_size, int parts, int rows_per_cta) {
-    const int per_row = 2 * NKV * hs / 8, part = blockIdx.x % parts;
-    const RowPlace me = row_place(hs, block_size, per_row, part, parts, rows_per_cta);
+    const int per_row = 2 * NKV * hs / kReadChannels, part = blockIdx.x % parts;
+    const RowPlace me = row_place(kReadChannels, hs, block_size, per_row, part, parts, rows_per_cta);
     pdl_wait();
     if (!me.active) return;
     const uint32_t page = (uint32_t)(2 * NKV) * block_size * (hs / kW4Group);
-    const long long step = (long long)(gridDim.x / parts) * rows_per_cta, ld = (long long)per_row * 8;
+    const long long step = (long long)(gridDim.x / parts) * rows_per_cta, ld = (long long)per_row * kReadChannels;
     const uint8_t* my_codes = codes + (size_t)me.group * (kW4Group / 2) + (me.col & (kW4Group - 1)) / 2;
     const uint32_t* my_scales = scales + me.group;
-    const unsigned sixteen = 0xffffu << (threadIdx.x & 16);
-    for (long long base = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; base < rows; base += 16 * step) {
-        const long long ahead = base + (threadIdx.x & 15) * step;
+    const unsigned eight = 0xffu << (threadIdx.x & 24);
+    for (long long base = (long long)(blockIdx.x / parts) * rows_per_cta + me.row; base < rows; base += 8 * step) {
+        const long long ahead = base + (threadIdx.x & 7) * step;
         const uint32_t place =
             ahead < rows ? slot_group(slot_map[ahead], slots, block_size, hs / kW4Group, page) : kNoRow;
         __nv_bfloat16* row = out + base * ld + me.col;
-        const int n = (int)min(16ll, (rows - base + step - 1) / step);
-        for (int k0 = 0; k0 < n; k0 += kRowsAhead) {
-            uint32_t word[kRowsAhead], meta[kRowsAhead];
+        const int n = (int)min(8ll, (rows - base + step - 1) / step);
+        for (int k0 = 0; k0 < n; k0 += kReadAhead) {
+            uint32_t word[kReadAhead], meta[kReadAhead];
 #pragma unroll
-            for (int k = 0; k < kRowsAhead; k++) {
-                const uint32_t at = __shfl_sync(sixteen, place, k0 + k, 16);
+            for (int k = 0; k < kReadAhead; k++) {
+                const uint32_t at = __shfl_sync(eight, place, k0 + k, 8);
                 word[k] = meta[k] = 0u;  // code 0, step 0, low end 0: zeros
                 if (at != kNoRow) {
                     word[k] = *reinterpret_cast<const uint32_t*>(my_codes + (size_t)at * (kW4Group / 2));
@@ -264,7 +273,7 @@ __global__ void __launch_bounds__(kRwThreads)
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kRowsAhead; k++) {
+            for (int k = 0; k < kReadAhead; k++) {
                 if (k0 + k < n) {
                     float x[8];
                     w4_values(word[k], meta[k], x);
@@ -283,19 +292,20 @@ __global__ void __launch_bounds__(kRwThreads)
 }
 
 // CTAs of a row pass: `parts` CTAs share a wide row, or a CTA takes `rows_per_cta` narrow ones; as many passes at
-// once as the rows give kRowsAhead each, at most 8 CTAs an SM.
+// once as the rows give `ahead` each, at most 4 CTAs an SM (what the append's registers allow: one wave; with 8
+// append and read-back of 16384 rows took 42.9 us together, with 4 41.3).
 struct RowGrid {
     int parts, rows_per_cta, grid;
 };
-static RowGrid row_grid(int rows, int NKV, int hs) {
-    const int per_row = 2 * NKV * hs / 8;
+static RowGrid row_grid(int rows, int NKV, int hs, int channels, int ahead) {
+    const int per_row = 2 * NKV * hs / channels;
     RowGrid g;
     g.parts = (per_row + kRwThreads - 1) / kRwThreads;
     g.rows_per_cta = g.parts > 1 ? 1 : kRwThreads / per_row;
     // few rows: a pass each, so that all of them are on their way at once
     long long passes = (rows + g.rows_per_cta - 1) / g.rows_per_cta;
-    const long long most = (long long)sm_count() * 8 / g.parts;
-    if (passes > most) passes = (passes + kRowsAhead - 1) / kRowsAhead;
+    const long long most = (long long)sm_count() * 4 / g.parts;
+    if (passes > most) passes = (passes + ahead - 1) / ahead;
     if (passes > most) passes = most;
     if (passes < 1) passes = 1;
     g.grid = (int)(passes * g.parts);
@@ -325,9 +335,9 @@ int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions,
                 blocks_have, free_list, free_count, B, max_blocks, block_size, max_rows, free_cap};
     static unsigned long long mask = 0;  // 4096 requests take 48 KB
     if (const cudaError_t e = ensure_smem_limit(block_tables_kernel, &mask)) return status_from(e);
-    long long grid = ((long long)max_rows + kTabThreads * 4 - 1) / (kTabThreads * 4);
+    long long grid = ((long long)max_rows + kTabThreads - 1) / kTabThreads;  // a row a thread, up to 2 CTAs an SM
     if (grid < 1) grid = 1;
-    if (grid > sm_count()) grid = sm_count();
+    if (grid > 2 * sm_count()) grid = 2 * sm_count();
     return status_from(launch_k(block_tables_kernel, dim3((unsigned)grid), dim3(kTabThreads), 3 * sizeof(int) * (size_t)B,
                                 (cudaStream_t)stream, true, a));
 }
@@ -354,7 +364,7 @@ int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_
     if (w4_too_large(NKV, hs, num_blocks, block_size)) return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(qkv) || ld % 8 != 0) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
-    const RowGrid g = row_grid(rows, NKV, hs);
+    const RowGrid g = row_grid(rows, NKV, hs, kWriteChannels, kWriteAhead);
     return status_from(launch_k(kv_write_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, true, kv_cache,
                                 (uint32_t*)kv_scale, (const __nv_bfloat16*)qkv, slot_map, rows, NH, NKV, hs, ld,
                                 (long long)num_blocks * block_size, block_size, g.parts, g.rows_per_cta));
@@ -368,7 +378,7 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
     if (w4_too_large(NKV, hs, num_blocks, block_size)) return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(out)) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
-    const RowGrid g = row_grid(rows, NKV, hs);
+    const RowGrid g = row_grid(rows, NKV, hs, kReadChannels, kReadAhead);
     return status_from(launch_k(kv_read_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, true,
                                 (__nv_bfloat16*)out, kv_cache, (const uint32_t*)kv_scale, slot_map, rows, NKV, hs,
                                 (long long)num_blocks * block_size, block_size, g.parts, g.rows_per_cta));
