@@ -84,6 +84,9 @@ float number(PyObject* o) {
 // elements between the rows of a 2-d tensor (its width where it has one row: the stride then says nothing)
 int pitch(const at::Tensor& t) { return size32(t.size(0) > 1 ? t.stride(0) : t.size(1), "a row pitch"); }
 
+// the same of 16-byte rows: a single row has no pitch that could be odd
+int qkv_pitch(const at::Tensor& t) { return t.size(0) > 1 ? pitch(t) : size32((t.size(1) + 7) / 8 * 8, "a row pitch"); }
+
 template <typename T> T* ptr(const at::Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 
 // The one CUDA device that holds every tensor, made current, and the stream to launch on.
@@ -186,7 +189,7 @@ PyObject* kv_cache_write_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Cache c = cache_of(a[0], a[1]);
         const at::Tensor& qkv = tensor(a[2], "qkv", at::kBFloat16, 2, true);
         const at::Tensor& slots = tensor(a[3], "slot_map", at::kLong, 1);
-        const int NH = integer(a[4], "NH"), rows = dim32(qkv, 0), ld = pitch(qkv);
+        const int NH = integer(a[4], "NH"), rows = dim32(qkv, 0), ld = qkv_pitch(qkv);
         if (slots.size(0) != rows || qkv.size(1) < ((int64_t)NH + 2 * c.NKV) * c.hs)
             refuse("slot_map has one entry a row, a row Q, K and V of every head");
         const Where w({&c.codes, &c.scales, &qkv, &slots}, a[5]);
@@ -223,7 +226,7 @@ PyObject* attention_forward_paged_w4(PyObject*, PyObject* const* a, Py_ssize_t n
         const at::Tensor& start = tensor(a[6], "row_start", at::kInt, 1);
         const int NH = integer(a[7], "NH"), max_q = integer(a[8], "max_q");
         const at::Tensor& ws = tensor(a[9], "workspace", at::kByte, 1);
-        const int rows = dim32(qkv, 0), ld = pitch(qkv), B = dim32(table, 0), max_blocks = dim32(table, 1);
+        const int rows = dim32(qkv, 0), ld = qkv_pitch(qkv), B = dim32(table, 0), max_blocks = dim32(table, 1);
         if (qkv.size(1) < ((int64_t)NH + 2 * c.NKV) * c.hs || out.size(0) != rows || out.size(1) != (int64_t)NH * c.hs)
             refuse("qkv is [rows, >= (NH + 2 NKV) hs] and out [rows, NH hs]");
         if (lens.size(0) != B || start.size(0) != (int64_t)B + 1) refuse("seq_lens has B entries and row_start B + 1");

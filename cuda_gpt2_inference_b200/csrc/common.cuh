@@ -294,6 +294,11 @@ inline cudaError_t ensure_smem_limit(Kernel k, unsigned long long* mask) {
     return e;
 }
 
+// Whether two byte ranges share a byte (an empty one or a null one shares none).
+inline bool ranges_overlap(const void* p, size_t n, const void* q, size_t m) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return p && q && n && m && a < b + m && b < a + n;
+}
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace gpt2b

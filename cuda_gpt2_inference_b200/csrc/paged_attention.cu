@@ -386,8 +386,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
             const int field = min(264 - (int)(__float_as_uint(mx) >> 23), 254);
             // the sign of the softmax scale goes to q, so that scores grow with S
             const float f = copysignf(pow2_field(field), a.scale_log2);
-            // D is in units of 2^-20 / f; never 0, so that a masked -infinity stays one
-            const float c = fmaxf(fabsf(a.scale_log2) * 1048576.0f * pow2_field(254 - field), 0x1p-120f);
+            // D is in units of 2^-20 / f; never 0 or infinite, so that a masked -infinity and a 0 stay ones
+            const float c = fminf(fmaxf(fabsf(a.scale_log2) * 1048576.0f * pow2_field(254 - field), 0x1p-120f), FLT_MAX);
             cf[nt][0] = __shfl_sync(0xffffffffu, c, 8 * t);
             cf[nt][1] = __shfl_sync(0xffffffffu, c, 8 * t + 4);
 #pragma unroll
@@ -870,6 +870,11 @@ int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const u
     int rc = gpt2b_attention_paged_w4_workspace(NH, NKV, hs, max_q, &need);
     if (rc) return rc;
     if (workspace_bytes < need || ((long long)NH + 2ll * NKV) * hs > ld) return GPT2B_ERR_INVALID_ARG;
+    if (!(scale >= -1e30f && scale <= 1e30f)) return GPT2B_ERR_INVALID_ARG;
+    const size_t out_bytes = (size_t)rows * NH * hs * 2;
+    if (rows > 0 && (ranges_overlap(out, out_bytes, qkv, ((size_t)(rows - 1) * ld + (size_t)(NH + 2 * NKV) * hs) * 2) ||
+                     ranges_overlap(workspace, need, out, out_bytes)))
+        return GPT2B_ERR_INVALID_ARG;
     // (positions are counted a few units past the end in 32 bits)
     if (block_size % kW4Tile != 0 || B > kTableMaxRequests || (long long)max_blocks * block_size > 1 << 30)
         return GPT2B_ERR_UNSUPPORTED;
@@ -877,7 +882,7 @@ int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const u
         ld % 8 != 0)
         return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
-    if ((long long)rows * NH > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
+    if ((long long)rows * NH > INT_MAX - 64) return GPT2B_ERR_UNSUPPORTED;
     if ((long long)NKV * block_size * hs > INT_MAX) return GPT2B_ERR_UNSUPPORTED;  // bytes of a block
     const PagedAttnArgs a{(__nv_bfloat16*)out, (const __nv_bfloat16*)qkv, kv_cache, (const uint32_t*)kv_scale, block_table,
                           seq_lens, row_start, B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks,

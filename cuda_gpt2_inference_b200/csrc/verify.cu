@@ -388,7 +388,12 @@ int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int 
     if (rows < 0 || V <= 0 || ld_logits < V || ld_probs < V || !(temperature == 0.0f || (temperature >= 1e-30f && temperature <= 1e30f)) ||
         (rows > 0 && (!probs || !logits)))
         return GPT2B_ERR_INVALID_ARG;
-    if (probs == logits && ld_logits != ld_probs) return GPT2B_ERR_INVALID_ARG;
+    if (rows > 0 && ranges_overlap(probs, ((size_t)(rows - 1) * ld_probs + V) * 4, logits, ((size_t)(rows - 1) * ld_logits + V) * 4)) {
+        // the same rows, or columns side by side in one buffer
+        const long long apart = ((long long)((intptr_t)probs - (intptr_t)logits) / 4 % ld_probs + ld_probs) % ld_probs;
+        const bool beside = apart >= V && apart + V <= ld_probs;
+        if (ld_probs != ld_logits || !(probs == logits || beside)) return GPT2B_ERR_INVALID_ARG;
+    }
     if (V > 1 << 30) return GPT2B_ERR_UNSUPPORTED;
     if (rows == 0) return GPT2B_OK;
     const int cluster = row_cluster(V, 16 * kProbThreads);
@@ -410,6 +415,10 @@ int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* token
         return GPT2B_ERR_INVALID_ARG;
     if (rows > 0 && (!tokens || !target_probs || !u_accept)) return GPT2B_ERR_INVALID_ARG;
     if (draft_probs && ld_draft < V) return GPT2B_ERR_INVALID_ARG;
+    const size_t out_bytes = 4 * (size_t)B * max_out, b4 = 4 * (size_t)B, r4 = 4 * (size_t)rows;
+    if (ranges_overlap(out_tokens, out_bytes, tokens, r4) || ranges_overlap(out_tokens, out_bytes, row_start, b4 + 4) ||
+        ranges_overlap(n_accepted, b4, tokens, r4) || ranges_overlap(n_accepted, b4, row_start, b4 + 4))
+        return GPT2B_ERR_INVALID_ARG;
     if (V > 1 << 30) return GPT2B_ERR_UNSUPPORTED;
     VerifyArgs a{out_tokens, n_accepted, tokens, target_probs, draft_probs, row_start, u_accept, u_sample,
                  B, rows, V, ld_target, ld_draft, max_out};

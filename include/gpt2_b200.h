@@ -260,8 +260,7 @@ int gpt2b_attention_forward_kv_large_bf16_noalloc(uint16_t* out, const uint16_t*
  *                     that is not served and behind the last request
  * and changes nothing else, so the same call again gives the same result; the
  * caller takes blocks_out and *free_left over as the next step's blocks_have and
- * *free_count.  These must be different buffers from the inputs
- * (GPT2B_ERR_INVALID_ARG).  free_cap is the length of free_list.  B <= 4096. */
+ * *free_count.  No output may overlap an input (GPT2B_ERR_INVALID_ARG).  free_cap is the length of free_list.  B <= 4096. */
 int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions, int* row_start, int* seq_lens,
                           int* blocks_out, int* free_left, const int* ctx_lens, const int* new_lens,
                           const int* blocks_have, const int* free_list, const int* free_count, int B, int max_blocks,
@@ -283,8 +282,8 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
  * drafts are causal among themselves.  out row: [NH*hs] BF16, zeros where a row
  * sees nothing.  seq_lens beyond max_blocks * block_size and row_start outside
  * [0, rows] are cut and reported (GPT2B_DEVERR_BAD_POS); a block outside the cache
- * is left out and reported (GPT2B_DEVERR_BAD_BLOCK).  scale: of the scores
- * (1/sqrt(hs)).  max_q: the most rows a request has, a hint for the tile choice.
+ * is left out and reported (GPT2B_DEVERR_BAD_BLOCK).  out overlaps neither qkv
+ * nor the workspace.  scale: of the scores (1/sqrt(hs)), at most 1e30.  max_q: the most rows a request has, a hint for the tile choice.
  * workspace: gpt2b_attention_paged_w4_workspace() bytes for the same NH, NKV, hs,
  * max_q on the current device, 16-byte aligned; needs no initialisation and holds
  * nothing between calls; calls that can overlap need one each.  B <= 4096,
@@ -343,7 +342,7 @@ int gpt2b_logits_nll(float* d_nll, const float* logits, int V, const int* d_toke
  * row (rows ld_* apart), FP32.  temperature is 0 or in [1e-30, 1e30]; 0: 1 at the largest logit (lowest
  * index on ties), 0 elsewhere.  A row with nothing above -infinity gives zeros; a
  * NaN or +infinity gives NaN (temperature 0 passes over NaN).  probs may be
- * logits.  No counterpart in the reference (its sampler keeps no probabilities). */
+ * logits (with the same ld), or other columns of the same rows; else they do not overlap.  No counterpart in the reference (its sampler keeps no probabilities). */
 int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int ld_logits, int ld_probs, float temperature,
                         gpt2b_stream_t stream);
 /* Verification of drafted tokens by rejection sampling.  Rows are packed as for
@@ -362,7 +361,8 @@ int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int 
  * out_tokens [B][max_out]: the accepted drafts, the drawn token, then -1; at most
  * max_out - 1 drafts are looked at.  n_accepted [B].  A request without rows gets
  * -1s and 0.  row_start outside [0, rows] is cut and reported
- * (GPT2B_DEVERR_BAD_POS).  No counterpart in the reference. */
+ * (GPT2B_DEVERR_BAD_POS).  The outputs overlap neither tokens nor row_start.  No
+ * counterpart in the reference. */
 int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* tokens, const float* target_probs,
                               const float* draft_probs, const int* row_start, const float* u_accept, const float* u_sample,
                               int B, int rows, int V, int ld_target, int ld_draft, int max_out, gpt2b_stream_t stream);

@@ -57,7 +57,7 @@ def attention(qkv, codes, scales, table, lens, start, NH, scale=None):
             # a score is a 32-bit sum of hs products of exact factors (hs + 8 roundings, of magnitude
             # |q||k|), twice (numerator and sum); a weight is held in 16 bits; e^x and the sums add
             # a few 32-bit roundings
-            sa = scale * torch.einsum("hrd,hpd->hrp", x.abs(), ka[:, :seen]).amax(-1, keepdim=True)
+            sa = abs(scale) * torch.einsum("hrd,hpd->hrp", x.abs(), ka[:, :seen]).amax(-1, keepdim=True)
             rel = 2 * (hs + 8) * 2.0 ** -24 * sa + FP16 + 2.0 ** -16
             mag = torch.einsum("hrp,hpd->hrd", w, va[:, :seen])
             # weights below 2^-18 of the largest step are held with an absolute error

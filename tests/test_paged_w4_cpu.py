@@ -20,7 +20,7 @@ def mem():
 
 def test_tables_refusals(gpt2b, mem):
     f, a = gpt2b.lib().gpt2b_kv_block_tables, mem
-    p = [a + 64 * i for i in range(12)]
+    p = [a + (i << 36) for i in range(12)]  # far apart, never read: these calls are refused
     ok = dict(B=2, mb=4, bs=16, rows=8, cap=4)
 
     def rc(ptrs=p, **kw):
@@ -31,9 +31,11 @@ def test_tables_refusals(gpt2b, mem):
         assert rc(**bad) == gpt2b.ERR_INVALID_ARG, bad
     for i in range(12):
         assert rc([None if k == i else x for k, x in enumerate(p)]) == gpt2b.ERR_INVALID_ARG, i
-    # results over inputs that every CTA reads
-    for dst, src in ((5, 9), (6, 11), (4, 7), (4, 8)):
-        assert rc([p[src] if k == dst else x for k, x in enumerate(p)]) == gpt2b.ERR_INVALID_ARG
+    # results over inputs that every CTA reads, as a whole or by a byte
+    for dst in range(7):
+        for src in range(7, 12):
+            assert rc([p[src] if k == dst else x for k, x in enumerate(p)]) == gpt2b.ERR_INVALID_ARG
+            assert rc([p[dst] + 3 if k == src else x for k, x in enumerate(p)]) == gpt2b.ERR_INVALID_ARG
     assert rc(B=4097) == gpt2b.ERR_UNSUPPORTED
     assert rc(mb=2 ** 28, bs=16) == gpt2b.ERR_UNSUPPORTED
 
@@ -72,18 +74,21 @@ def test_attention_refusals(gpt2b, mem):
         assert size(NH, NKV, hs, q, ctypes.byref(n)) == gpt2b.ERR_INVALID_ARG
     assert size(4, 2, 80, 1, ctypes.byref(n)) == gpt2b.ERR_UNSUPPORTED
 
-    def rc(out=a, qkv=a, codes=a, scales=a, table=a, lens=a, start=a, B=1, rows=1, NH=2, NKV=2, hs=64, ld=384, nb=2, bs=16,
-           mb=2, q=1, ws=a, bytes=1 << 40):
+    far = 1 << 44
+
+    def rc(out=a + far, qkv=a, codes=a, scales=a, table=a, lens=a, start=a, B=1, rows=1, NH=2, NKV=2, hs=64, ld=384, nb=2, bs=16,
+           mb=2, q=1, ws=a + 2 * far, bytes=1 << 40, scale=0.125):
         return lib.gpt2b_attention_forward_paged_w4(out, qkv, codes, scales, table, lens, start, B, rows, NH, NKV, hs, ld, nb,
-                                                    bs, mb, q, 0.125, ws, bytes, None)
+                                                    bs, mb, q, scale, ws, bytes, None)
 
     for bad in (dict(out=None), dict(qkv=None), dict(codes=None), dict(scales=None), dict(table=None), dict(lens=None),
                 dict(start=None), dict(ws=None), dict(B=0), dict(rows=-1), dict(NH=3), dict(NKV=0), dict(nb=0), dict(bs=0),
-                dict(mb=0), dict(q=0), dict(bytes=0), dict(ld=383)):
+                dict(mb=0), dict(q=0), dict(bytes=0), dict(ld=383), dict(out=a), dict(out=a + 16, rows=3), dict(ws=a + far),
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=-2e30)):
         assert rc(**bad) == gpt2b.ERR_INVALID_ARG, bad
     for bad in (dict(hs=32), dict(bs=8), dict(B=4097), dict(mb=2 ** 28)):
         assert rc(**{"ld": 4096, **bad}) == gpt2b.ERR_UNSUPPORTED, bad
-    for bad in (dict(out=a + 8), dict(qkv=a + 2), dict(codes=a + 1), dict(scales=a + 4), dict(ws=a + 4), dict(ld=388)):
+    for bad in (dict(out=a + far + 8), dict(qkv=a + 2), dict(codes=a + 1), dict(scales=a + 4), dict(ws=a + 2 * far + 4), dict(ld=388)):
         assert rc(**bad) == gpt2b.ERR_ALIGNMENT, bad
     assert rc(rows=0) == gpt2b.OK
 
@@ -96,15 +101,16 @@ def test_probs_and_verify_refusals(gpt2b, mem):
         return lib.gpt2b_softmax_probs(out, x, rows, V, li, lo, T, None)
 
     for bad in (dict(out=None), dict(x=None), dict(rows=-1), dict(V=0), dict(li=7), dict(lo=7), dict(T=-1.0), dict(T=nan), dict(T=1e-31), dict(T=1e31),
-                dict(T=inf), dict(li=9)):
+                dict(T=inf), dict(li=9), dict(out=a + 4), dict(out=a + 32, rows=2), dict(out=a + 36, rows=2, li=16, lo=16)):
         assert probs(**bad) == gpt2b.ERR_INVALID_ARG, bad
     assert probs(rows=0) == gpt2b.OK
 
-    def verify(out=a, n=a, tok=a, p=a, q=a, start=a, ua=a, us=a, B=1, rows=2, V=8, lp=8, lq=8, width=3):
+    def verify(out=a, n=a + (1 << 40), tok=a + (2 << 40), p=a, q=a, start=a + (3 << 40), ua=a, us=a, B=1, rows=2, V=8, lp=8, lq=8, width=3):
         return lib.gpt2b_verify_draft_tokens(out, n, tok, p, q, start, ua, us, B, rows, V, lp, lq, width, None)
 
     for bad in (dict(out=None), dict(n=None), dict(tok=None), dict(p=None), dict(start=None), dict(ua=None), dict(us=None),
-                dict(B=0), dict(rows=-1), dict(V=0), dict(lp=7), dict(lq=7), dict(width=0)):
+                dict(B=0), dict(rows=-1), dict(V=0), dict(lp=7), dict(lq=7), dict(width=0), dict(out=a + (2 << 40)),
+                dict(n=a + (2 << 40) + 4), dict(out=a + (3 << 40)), dict(n=a + (3 << 40)), dict(tok=a + 8)):
         assert verify(**bad) == gpt2b.ERR_INVALID_ARG, bad
 
 

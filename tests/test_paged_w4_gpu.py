@@ -519,3 +519,16 @@ def test_attention_of_two_calls_at_once(cuda):
     torch.cuda.synchronize()
     for k in range(2):
         assert all(torch.equal(o, want[k]) for o in outs[k])
+
+
+def test_single_row_of_any_width_and_negative_scale(cuda):
+    from cuda_gpt2_inference_b200 import ops
+    st = _attention_state(2, 1, 64, 16, [50], [1], 51, pad=0)
+    NH, qkv, codes, scales, table, lens, start = st
+    _check_attention(st, _attend(st, 1, scale=-0.25), scale=-0.25)
+    _check_attention(st, _attend(st, 1, scale=0.0), scale=0.0)
+    odd = torch.cat([qkv, torch.zeros(1, 3, dtype=BF)], 1).cuda()  # one row has no pitch that could be odd
+    ws = torch.empty(ops.attention_paged_w4_workspace(2, 2, 64, 1), dtype=torch.uint8, device="cuda")
+    out = torch.zeros(1, 128, dtype=BF, device="cuda")
+    ops.attention_forward_paged_w4(out, odd, codes.cuda(), scales.cuda(), table.cuda(), lens.cuda(), start.cuda(), 2, 1, ws)
+    assert torch.equal(out, _attend(st, 1))

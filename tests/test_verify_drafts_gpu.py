@@ -206,3 +206,15 @@ def test_verify_in_a_graph(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert (out.tolist(), n.tolist()) == plain.verify(tokens, probs.cpu(), q, start, ua2.cpu(), us, 7)
+
+
+def test_probs_beside_their_logits(cuda):
+    """Logits and probabilities as columns of one buffer."""
+    from cuda_gpt2_inference_b200 import ops
+    both = torch.zeros(7, 2 * 333 + 5, device="cuda")
+    x = torch.randn(7, 333, generator=torch.Generator().manual_seed(3))
+    both[:, :333] = x.cuda()
+    ops.softmax_probs(both[:, 336:669], both[:, :333])
+    want = torch.softmax(x.double(), -1)
+    assert ((both[:, 336:669].cpu().double() - want).abs() <= 2.0 ** -20 * want).all()
+    assert torch.equal(both[:, :333].cpu(), x) and not both[:, 333:336].any() and not both[:, 669:].any()
