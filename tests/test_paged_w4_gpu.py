@@ -532,3 +532,76 @@ def test_single_row_of_any_width_and_negative_scale(cuda):
     out = torch.zeros(1, 128, dtype=BF, device="cuda")
     ops.attention_forward_paged_w4(out, odd, codes.cuda(), scales.cuda(), table.cuda(), lens.cuda(), start.cuda(), 2, 1, ws)
     assert torch.equal(out, _attend(st, 1))
+
+
+def test_drafted_decoding_of_a_batch(cuda, gpt2b):
+    """Six steps of drafted decoding as one would write them: lengths, tables and cache are carried on the device,
+    refused drafts are overwritten, a request without drafts stands beside others.  A stand-in for the model (token
+    and position embeddings to q, k, v; attention to logits) keeps the rows' contents honest."""
+    from cuda_gpt2_inference_b200 import ops
+    NKV, NH, hs, bs, nb, mb, B, V, width = 2, 4, 64, 16, 40, 12, 3, 300, 5
+    cap, T = B * width, 0.8
+    g = torch.Generator().manual_seed(77)
+    emb = torch.randn(V + 400, (NH + 2 * NKV) * hs, generator=g).to(BF).cuda()
+    head = (torch.randn(NH * hs, V, generator=g) * 0.3).to(BF).cuda()
+    codes = torch.zeros(nb, 2, NKV, bs, hs // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.full((nb, 2, NKV, bs, 1, 2), math.nan, dtype=BF, device="cuda")
+    table = torch.full((B, mb), -1, dtype=I32, device="cuda")
+    free, count, have, ctx = i32(list(range(nb))), i32([nb]), i32([0] * B), i32([0] * B)
+    slot, pos = torch.empty(cap, dtype=I64, device="cuda"), torch.empty(cap, dtype=I32, device="cuda")
+    start, lens, blocks, left = i32([0] * (B + 1)), i32([0] * B), i32([0] * B), i32([0])
+    atty = torch.zeros(cap, NH * hs, dtype=BF, device="cuda")
+    probs = torch.zeros(cap, V, device="cuda")
+    out, taken = torch.zeros(B, width, dtype=I32, device="cuda"), torch.zeros(B, dtype=I32, device="cuda")
+    ws = torch.empty(ops.attention_paged_w4_workspace(NH, NKV, hs, width), dtype=torch.uint8, device="cuda")
+    seqs = [[5], [7], [9]]                      # what each request has said so far, the last token not yet cached
+    drafts_of = [4, 0, 2]
+    told = 0
+    for step in range(6):
+        dp = torch.softmax(torch.randn(cap, V, generator=g), -1)
+        rows, tokens = [], []
+        for b in range(B):
+            guess = torch.multinomial(dp[len(tokens):len(tokens) + max(1, drafts_of[b])], 1, generator=g)[:, 0].tolist()
+            row = [seqs[b][-1]] + guess[:drafts_of[b]]
+            rows.append(len(row))
+            tokens += row
+        tokens += [0] * (cap - len(tokens))
+        dtok, ua, us = i32(tokens), torch.rand(cap, generator=g) * 0.2, torch.rand(B, generator=g)
+        ops.kv_block_tables(table, slot, pos, start, lens, blocks, left, ctx, i32(rows), have, free, count, bs)
+        qkv = emb[dtok.long()] + emb[V + pos.long()]
+        ops.kv_cache_write_w4(codes, scales, qkv, slot, NH)
+        ops.attention_forward_paged_w4(atty, qkv, codes, scales, table, lens, start, NH, width, ws)
+        logits = (atty @ head).float()
+        ops.softmax_probs(probs, logits, T)
+        ops.verify_draft_tokens(out, taken, dtok, probs, dp.cuda(), start, ua.cuda(), us.cuda())
+        # what it should have been: the request's whole text, quantised position by position
+        st = start.tolist()
+        n_ctx = [len(s) - 1 for s in seqs]
+        assert lens.tolist() == [c + r for c, r in zip(n_ctx, rows)]
+        flat_c, flat_s, tabs = [], [], []
+        for b in range(B):
+            text = seqs[b][:-1] + tokens[st[b]:st[b + 1]]
+            x = emb[torch.tensor(text).cuda()] + emb[V + torch.arange(len(text)).cuda()]
+            kv = x[:, NH * hs:].cpu().view(-1, 2, NKV, hs)
+            kv = torch.cat([kv, torch.zeros(-len(text) % bs, 2, NKV, hs, dtype=BF)])
+            c, s = plain.quantise(kv.view(-1, bs, 2, NKV, hs).permute(0, 2, 3, 1, 4))
+            tabs.append(list(range(sum(map(len, flat_c)), sum(map(len, flat_c)) + len(c))))
+            flat_c.append(c)
+            flat_s.append(s)
+        wide = max(map(len, tabs))
+        pt = torch.tensor([t + [0] * (wide - len(t)) for t in tabs], dtype=I32)
+        want, err = plain.attention(qkv.cpu(), torch.cat(flat_c), torch.cat(flat_s), pt, lens.cpu(), start.cpu(), NH)
+        R = st[-1]
+        assert ((atty[:R].cpu().double() - want[:R]).abs() <= plain.BF16 * want[:R].abs() + 1.01 * err[:R] + 2.0 ** -126).all()
+        ref = torch.softmax(logits[:R].cpu().double() / T, -1)
+        assert ((probs[:R].cpu().double() - ref).abs() <= 2.0 ** -17 * ref + 2.0 ** -126).all()
+        assert (out.tolist(), taken.tolist()) == plain.verify(torch.tensor(tokens), probs.cpu(), dp, st, ua, us, width)
+        for b in range(B):
+            got = [t for t in out[b].tolist() if t >= 0]
+            assert len(got) == int(taken[b]) + 1
+            seqs[b] += got
+            told += int(taken[b])
+        ctx.add_(taken).add_(1)
+        have.copy_(blocks)
+        count.copy_(left)
+    assert told > 0 and gpt2b.device_error() == 0
