@@ -142,6 +142,11 @@ __device__ __forceinline__ void pa_scan(const PagedAttnArgs& a, int cols, long l
         __syncthreads();
     }
 }
+// where the run of CTA i of G begins: total * i / G, in 32 bits where that does (a 64-bit division takes longer than
+// the loads around it)
+__device__ __forceinline__ long long pa_run(long long total, int i, int G) {
+    return total < (1 << 20) && G < 4096 ? (long long)((unsigned)total * (unsigned)i / (unsigned)G) : total * i / G;
+}
 // the request that holds unit u
 __device__ __forceinline__ int pa_find(const long long* pre, int B, long long u) {
     int lo = 0, hi = B - 1;
@@ -242,10 +247,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
     pdl_trigger();  // the joining launch may wait on the SMs as they become free
     pa_scan(a, COLS, pre, wsum, blockIdx.x == 0);
     const long long total = pre[a.B];
-    const long long G = min((long long)gridDim.x, total);
-    if (blockIdx.x >= G) return;
-    long long u = total * blockIdx.x / G;
-    const long long u_end = total * (blockIdx.x + 1) / G;
+    const int G = (int)min((long long)gridDim.x, total);
+    if ((int)blockIdx.x >= G) return;
+    long long u = pa_run(total, blockIdx.x, G);
+    const long long u_end = pa_run(total, blockIdx.x + 1, G);
     int b = pa_find(pre, a.B, u);
 
     // this lane's places in a stage
@@ -750,14 +755,14 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
     long long* pre = reinterpret_cast<long long*>(smem);
     __shared__ long long wsum[kPaWarps];
     pa_scan(a, COLS, pre, wsum, false);
-    const long long total = pre[a.B], G = min((long long)main_grid, total);
-    const long long i0 = blockIdx.x;
+    const long long total = pre[a.B];
+    const int G = (int)min((long long)main_grid, total), i0 = blockIdx.x;
     const int ratio = a.NH / a.NKV;
     bool mine = false;
     int b = 0, kvh = 0, chunk = 0, pieces = 0;
     PaRequest rq{};
     if (i0 + 1 < G) {
-        const long long u = total * (i0 + 1) / G;
+        const long long u = pa_run(total, i0 + 1, G);
         b = pa_find(pre, a.B, u);
         rq = pa_request(a, b, COLS, false);
         const PaPlace pl = pa_place(rq, u - pre[b]);
