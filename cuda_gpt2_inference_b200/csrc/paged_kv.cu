@@ -24,6 +24,9 @@ GPT2B_DEFINE_ERROR_READER(paged_kv_device_error)
 // 12 bytes a request from L2 against a second launch.  Nothing that a CTA reads
 // is written by another: a row's block is either one that the request held
 // (below have, which no CTA writes) or comes from the free list directly.
+// Bound by its launch and the chain lengths - scan - block - store: 2.7 us for 8
+// requests of one row, 3.7 us for 256 with 64000 rows (a row a thread; with four rows
+// a thread in a quarter of the CTAs 5.9 us).
 constexpr int kTabThreads = 256;
 
 struct TableArgs {
