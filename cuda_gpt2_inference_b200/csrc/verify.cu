@@ -73,10 +73,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // One CTA of a row's cluster takes a contiguous part of it.  A thread keeps a running maximum and a sum about it,
 // a warp joins its threads', and the pairs (m, sum) of all the cluster's warps are exchanged behind its one
 // barrier.  Then each thread reads its entries again, from L1 or L2 (unless one batch of loads was all), and writes
-// e^((x - M)/T) / total.  Nothing is kept in between, so 6 CTAs of 256 threads fit an SM and their loads, exchanges and stores overlap: 320 x 50257
-// takes 35 us, against 38 with the entries kept in registers (3 CTAs of 512 an SM) and 53 with those and the
-// next row's.  8 bytes an entry from and to HBM bound it (19.7 us).  Few rows: 512 threads with all loads in
-// flight at once; there the chain launch - load - exchange - store is what counts.
+// e^((x - M)/T) / total.  Nothing is kept in between, so 6 CTAs of 256 threads fit an SM and their loads, exchanges
+// and stores overlap: 320 x 50257 takes 35 us (3.6 TB/s), against 38 with the entries kept in registers (3 CTAs of
+// 512 an SM) and 53 with those and the next row's.  HBM, 8 bytes an entry, would take 19.7; what keeps it from that
+// is the chain load - exchange - store of each row.  Few rows: 512 threads with all loads in flight at once; there
+// launch and chain are all (5 rows: 3.7 us on the device).
 struct ProbPart {
     float m, s;
 };

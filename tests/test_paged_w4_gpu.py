@@ -605,3 +605,22 @@ def test_drafted_decoding_of_a_batch(cuda, gpt2b):
         have.copy_(blocks)
         count.copy_(left)
     assert told > 0 and gpt2b.device_error() == 0
+
+
+def test_attention_of_many_and_of_no_requests(cuda, gpt2b):
+    """As many requests as a call takes, most of them with nothing cached or nothing asked; and none with rows."""
+    lens, rows = [k % 4 for k in range(4096)], [k % 3 for k in range(4096)]
+    st = _attention_state(1, 2, 64, 16, lens, rows, 61)
+    _check_attention(st, _attend(st, 2))
+    st = _attention_state(2, 1, 128, 16, [20, 0, 7], [0, 0, 0], 62)
+    out = _attend(st, 1)
+    assert (out == 123.0).all()
+    assert gpt2b.device_error() == 0
+
+
+def test_attention_of_one_long_request_over_one_head(cuda):
+    """The whole GPU on one segment: more pieces to join than one pass of the join takes."""
+    st = _attention_state(1, 2, 128, 64, [70001], [1], 63)
+    _check_attention(st, _attend(st, 1))
+    st = _attention_state(1, 1, 64, 16, [30011], [17], 64)
+    _check_attention(st, _attend(st, 17))
