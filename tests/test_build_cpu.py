@@ -1,4 +1,4 @@
-"""The checker's build step where the reference checkout is absent."""
+"""The oracle's build step where the reference checkout is absent."""
 from __future__ import annotations
 
 import pytest

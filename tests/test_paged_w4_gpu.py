@@ -171,6 +171,8 @@ CASES = [  # NKV, ratio, hs, bs, lens, rows
     (2, 1, 128, 16, [40, 90], [40, 17]),                    # a prompt without a past
     (1, 1, 64, 16, [5000], [2]),
     (1, 4, 128, 32, [9001], [1]),
+    (2, 1, 64, 96, [500, 97, 96, 95], [2, 1, 1, 3]),
+    (1, 3, 128, 160, [1000, 161, 31], [7, 1, 2]),
     (1, 1, 64, 16, list(range(0, 300)), [1] * 300),         # more requests than a pass of the CTA's scan
 ]
 
