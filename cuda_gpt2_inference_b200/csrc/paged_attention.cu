@@ -24,8 +24,8 @@
 // What bounds it: instruction issue.  A step of 32 positions of 128 channels takes a warp
 // about 540 instructions, half of them on the ALU pipe (decode, steps, maxima), which the
 // SM issues at 55 % of its rate; HBM would need 63 % of the time.  Measured, of the 6.54 TB/s
-// of a copy: 32 x 16384 positions of 8 heads of 128, one row of 4 query heads each: 127 us,
-// 73 %; 16 columns: 170 us, 54 %; 32 x 8192 of 25 heads of 64, one row: 106 us, 68 %.  One
+// of a copy: 32 x 16384 positions of 8 heads of 128, one row of 4 query heads each: 125 us,
+// 74 %; 16 columns: 175 us, 53 %; 32 x 8192 of 25 heads of 64, one row: 105 us, 69 %.  One
 // request of 1001 positions and 12 heads: 6 us, a chain of launch, lengths, table, codes, join.
 #include "paged_kv.cuh"
 #include "internal.h"
@@ -76,6 +76,9 @@ template <int NG, int NT> struct PaShape {
     // (18.5 against 19.4 us at 16 x 1024).
     static constexpr int kCtas = NG * NT == 1 ? 4 : NG * NT == 2 ? 3 : 2;
     static constexpr int kSlot = kCols * (kHS + 2);                 // floats of a partial result
+    // Scores and low ends two columns an instruction (us at the sizes above): hs 128 with 8 columns 129 -> 125,
+    // hs 64 with 16 columns 153 -> 150, with 8 the same; hs 128 with 16 columns 174 -> 183, so not there.
+    static constexpr bool kPacked = NG * NT <= 2;
 };
 
 // ---------------------------------------------------------------------------
@@ -507,12 +510,24 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int k = 0; k < 2; k++) {
                         const float ks = meta_step(km[j][k][ng]), kz = meta_low(km[j][k][ng]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                        for (int nt = 0; nt < NT; nt++) {
+                            if constexpr (Sh::kPacked) {
+                                float z0, z1;
+                                if (ng == 0) {
+                                    z0 = kz * qs[nt][0][0];
+                                    z1 = kz * qs[nt][0][1];
+                                } else {
+                                    fma2(z0, z1, kz, kz, qs[nt][ng][0], qs[nt][ng][1], S[j][nt][2 * k], S[j][nt][2 * k + 1]);
+                                }
+                                fma2(S[j][nt][2 * k], S[j][nt][2 * k + 1], ks, ks, D[j][nt][2 * k], D[j][nt][2 * k + 1], z0, z1);
+                            } else {
 #pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                const float z = ng == 0 ? kz * qs[nt][0][c] : fmaf(kz, qs[nt][ng][c], S[j][nt][2 * k + c]);
-                                S[j][nt][2 * k + c] = fmaf(ks, D[j][nt][2 * k + c], z);
+                                for (int c = 0; c < 2; c++) {
+                                    const float z = ng == 0 ? kz * qs[nt][0][c] : fmaf(kz, qs[nt][ng][c], S[j][nt][2 * k + c]);
+                                    S[j][nt][2 * k + c] = fmaf(ks, D[j][nt][2 * k + c], z);
+                                }
                             }
+                        }
                     }
             }
             if constexpr (MASKED) {  // positions that a column does not see
@@ -637,12 +652,18 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                         for (int k = 0; k < 2; k++) {
                             const float vs = meta_step(vm[j][k][ng]), vz = meta_low(vm[j][k][ng]);
                             float x[2];
+                            if constexpr (!MASKED && Sh::kPacked) {
+                                x[0] = p[2 * k] * vs;
+                                x[1] = p[2 * k + 1] * vs;
+                                fma2(az[nt][ng][0], az[nt][ng][1], p[2 * k], p[2 * k + 1], vz, vz, az[nt][ng][0], az[nt][ng][1]);
+                            } else {
 #pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                // a position that this column does not see may hold NaN, and 0 * NaN is not 0
-                                const bool hidden = MASKED && S[j][nt][2 * k + c] == -INFINITY;
-                                x[c] = hidden ? 0.0f : p[2 * k + c] * vs;
-                                az[nt][ng][c] = hidden ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
+                                for (int c = 0; c < 2; c++) {
+                                    // a position that this column does not see may hold NaN, and 0 * NaN is not 0
+                                    const bool hidden = MASKED && S[j][nt][2 * k + c] == -INFINITY;
+                                    x[c] = hidden ? 0.0f : p[2 * k + c] * vs;
+                                    az[nt][ng][c] = hidden ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
+                                }
                             }
                             wb[nt][ng][k] = mov_trans(f16x2(x[0], x[1]));
                         }
