@@ -135,12 +135,14 @@ template <typename F> PyObject* entry(const char* where, Py_ssize_t want, Py_ssi
     }
     return nullptr;
 }
+// Without the interpreter lock, which comes back however f is left (a size or a data pointer may be refused in it).
+struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
 template <typename F> int launch(F&& f) {
-    int status;
-    Py_BEGIN_ALLOW_THREADS
-    status = f();
-    Py_END_ALLOW_THREADS
-    return status;
+    const Unlocked u;
+    return f();
 }
 
 struct Cache {

@@ -218,3 +218,20 @@ def test_probs_beside_their_logits(cuda):
     want = torch.softmax(x.double(), -1)
     assert ((both[:, 336:669].cpu().double() - want).abs() <= 2.0 ** -20 * want).all()
     assert torch.equal(both[:, :333].cpu(), x) and not both[:, 333:336].any() and not both[:, 669:].any()
+
+
+def test_sizes_beyond_32_bits_are_refused(cuda, gpt2b):
+    """Empty tensors hold no memory and may have any size; the refusal is an error of the call, which the next
+    call does not see."""
+    from cuda_gpt2_inference_b200 import ops
+    many = torch.empty(2 ** 31, 0, device=cuda)
+    with pytest.raises(gpt2b.Gpt2bError, match="32 bits"):
+        ops.softmax_probs(many, many, V=0)
+    one = torch.empty(0, dtype=torch.int32, device=cuda)
+    with pytest.raises(gpt2b.Gpt2bError, match="32 bits"):
+        ops.verify_draft_tokens(torch.empty(0, 2 ** 31, dtype=torch.int32, device=cuda), one, one,
+                                torch.empty(0, 8, device=cuda), None, torch.zeros(1, dtype=torch.int32, device=cuda),
+                                one.float(), one.float())
+    logits = torch.zeros(1, 4, device=cuda)
+    ops.softmax_probs(logits, logits)
+    assert logits.tolist() == [[0.25] * 4]
