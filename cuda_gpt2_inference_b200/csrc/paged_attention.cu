@@ -55,6 +55,9 @@ constexpr int kPaWarps = 4, kPaThreads = 32 * kPaWarps;
 constexpr int kPaStep = 32;                  // positions a warp takes at a time
 constexpr int kPaUnit = kPaStep * kPaWarps;  // positions of a unit of the work partition
 constexpr int kPaExtra = 2;                  // what a segment costs beside its units, in units
+// Weights are 2^(score - running maximum - kBias): their sums, up to 2^8 a position, then reach 2^24 positions before
+// a product with a value of FP32's whole range overflows, and a weight underflows only 2^-100 below the largest.
+constexpr float kBias = 24.0f;
 
 // NG groups of 64 channels, NT tiles of 8 columns.
 template <int NG, int NT> struct PaShape {
@@ -233,6 +236,8 @@ template <int NG> __device__ __forceinline__ void lds_meta(uint32_t addr, uint32
 __device__ __forceinline__ float meta_step(uint32_t m) { return __uint_as_float(m << 16); }
 __device__ __forceinline__ float meta_low(uint32_t m) { return __uint_as_float(m & 0xffff0000u); }
 __device__ __forceinline__ float pow2_field(int field) { return __uint_as_float((uint32_t)field << 23); }
+
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
 constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // nibbles as code * 2^-24 / code * 2^-20
 
@@ -456,10 +461,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int k = 0; k < 4; k++) acc[nt][ng][i][k] = 0.0f;
             }
         }
-        // What the weights are summed with: l, az and acc carry a factor 2^s_shift that brings V's steps, as
-        // long as they do not pass s_lim, into FP16's range
-        float s_lim = -1.0f;
-        int s_shift = 0;
+        // acc carries a factor `vscale`, a power of two that brings V's steps below 2^31: with the weights, at most
+        // 2^(8 - kBias), they stay below 2^15, in FP16's range.  l and az have no part in it: low ends have a range
+        // of their own.
+        float vscale = 0x1p124f;
 
         auto step = [&](auto mask_tag, int p0, uint32_t base, uint32_t badbits) {
             constexpr bool MASKED = decltype(mask_tag)::value;
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                         big = fmaxf(big, fabsf(meta_step(vm[j][k][ng])));
                     }
                 }
-            if (__any_sync(0xffffffffu, big > s_lim)) {
+            if (__any_sync(0xffffffffu, big * vscale >= 0x1p31f)) {
                 // a step beyond what the factor allows: take the warp's largest finite one
                 big = 0.0f;
 #pragma unroll
@@ -602,29 +607,19 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                             if (x < INFINITY) big = fmaxf(big, x);
                         }
                 big = warp_max(big);
-                if (big > s_lim) {
-                    // largest step -> [2^4, 2^5), with room for two exponents of growth: operands below 2^15.
-                    // The factor itself stays below 2^100, so that FP32 holds the sums that carry it.
-                    const int ef = (int)(__float_as_uint(big) >> 23);
-                    const int shift = big == 0.0f ? 0 : min(131 - ef, 100);
-                    const float f = pow2_field(max(127 + shift - s_shift, 0));
+                if (big * vscale >= 0x1p31f) {
+                    // largest step -> [2^28, 2^29), with room for two exponents of growth
+                    const float next = pow2_field(282 - (int)(__float_as_uint(big) >> 23));
+                    const float f = next * pow2_inverse(vscale);
+                    vscale = next;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            l[nt][c] *= f;
+                        for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-                            for (int ng = 0; ng < NG; ng++) {
-                                az[nt][ng][c] *= f;
+                            for (int i = 0; i < 4; i++)
 #pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    acc[nt][ng][i][c] *= f;
-                                    acc[nt][ng][i][c + 2] *= f;
-                                }
-                            }
-                        }
-                    s_shift = shift;
-                    s_lim = big == 0.0f ? 0.0f : __uint_as_float((uint32_t)(min(ef + 2, 254)) << 23 | 0x7fffffu);
+                                for (int k = 0; k < 4; k++) acc[nt][ng][i][k] *= f;
                 }
             }
             // ---- weights (FP32 statistics, FP16 operands) and out += codes_V^T . weights
@@ -632,7 +627,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) off[nt][c] = (float)s_shift - m[nt][c];
+                for (int c = 0; c < 2; c++) off[nt][c] = -kBias - m[nt][c];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 uint32_t wb[NT][NG][2];
@@ -650,7 +645,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int ng = 0; ng < NG; ng++) {
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
-                            const float vs = meta_step(vm[j][k][ng]), vz = meta_low(vm[j][k][ng]);
+                            const float vs = meta_step(vm[j][k][ng]) * vscale, vz = meta_low(vm[j][k][ng]);
                             float x[2];
                             if constexpr (!MASKED && Sh::kPacked) {
                                 x[0] = p[2 * k] * vs;
@@ -720,7 +715,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 if (g == 0) s_m[w * COLS + nt * 8 + 2 * t + c] = m[nt][c];
             }
         __syncthreads();
-        const float unscale = pow2_field(127 - s_shift);
+        const float even = 16777216.0f * pow2_inverse(vscale), odd = 1048576.0f * pow2_inverse(vscale);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -729,15 +724,15 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 float M = s_m[col];
                 for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
                 const float f = ex2(m[nt][c] - M);  // 1 where nothing was seen: zeros (or NaN) are joined
-                if (g == 0) s_l[w * COLS + col] = l[nt][c] * unscale * f;
+                if (g == 0) s_l[w * COLS + col] = l[nt][c] * f;
                 float* dst = slab + (w * COLS + col) * Sh::kPitch;
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int ch = ng * kW4Group + 8 * g + 2 * i;
-                        dst[ch] = fmaf(acc[nt][ng][i][c], 16777216.0f, az[nt][ng][c]) * unscale * f;
-                        dst[ch + 1] = fmaf(acc[nt][ng][i][c + 2], 1048576.0f, az[nt][ng][c]) * unscale * f;
+                        dst[ch] = fmaf(acc[nt][ng][i][c], even, az[nt][ng][c]) * f;
+                        dst[ch + 1] = fmaf(acc[nt][ng][i][c + 2], odd, az[nt][ng][c]) * f;
                     }
             }
         __syncthreads();
