@@ -461,10 +461,14 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int k = 0; k < 4; k++) acc[nt][ng][i][k] = 0.0f;
             }
         }
-        // acc carries a factor `vscale`, a power of two that brings V's steps below 2^31: with the weights, at most
-        // 2^(8 - kBias), they stay below 2^15, in FP16's range.  l and az have no part in it: low ends have a range
-        // of their own.
-        float vscale = 0x1p124f;
+        // A column's acc carries its `vscale`, a power of two that brings the V steps that the column sees below
+        // 2^31: with the weights, at most 2^(8 - kBias), they stay below 2^15, in FP16's range.  Steps that it does
+        // not see have no part in it, or a later row's outlier would take bits from an earlier row.  Only masked steps
+        // make columns differ, and what follows a step that some columns do not see is masked too, so unmasked ones
+        // find the same vscale everywhere.  l and az have no factor: low ends have a range of their own.
+        float vscale[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) vscale[nt][0] = vscale[nt][1] = 0x1p124f;
 
         auto step = [&](auto mask_tag, int p0, uint32_t base, uint32_t badbits) {
             constexpr bool MASKED = decltype(mask_tag)::value;
@@ -579,48 +583,52 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                         }
                     }
             }
-            // ---- V steps; those of positions that no column sees may be anything
+            // ---- V steps; a column's largest where it passes what the column's factor allows
             uint32_t vm[2][2][NG];
-            float big = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    lds_meta<NG>(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG), vm[j][k]);
-                    const bool none = MASKED && (p0 + 16 * j + tile_pos(g) + 8 * k >= p_end || ((badbits >> j) & 1u));
-#pragma unroll
-                    for (int ng = 0; ng < NG; ng++) {
-                        if (none) vm[j][k][ng] = 0;
-                        big = fmaxf(big, fabsf(meta_step(vm[j][k][ng])));
-                    }
-                }
-            if (__any_sync(0xffffffffu, big * vscale >= 0x1p31f)) {
-                // a step beyond what the factor allows: take the warp's largest finite one
-                big = 0.0f;
+                for (int k = 0; k < 2; k++) lds_meta<NG>(mbase + Sh::kMetaBytes + j * (64 * NG) + k * (32 * NG), vm[j][k]);
+            auto largest = [&](int nt, int c, bool finite) {  // of this lane's positions that the column sees
+                float big = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int ng = 0; ng < NG; ng++)
+                    for (int k = 0; k < 2; k++)
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
+                        for (int ng = 0; ng < NG; ng++) {
                             const float x = fabsf(meta_step(vm[j][k][ng]));
-                            if (x < INFINITY) big = fmaxf(big, x);
+                            if ((!MASKED || S[j][nt][2 * k + c] != -INFINITY) && (!finite || x < INFINITY)) big = fmaxf(big, x);
                         }
-                big = warp_max(big);
-                if (big * vscale >= 0x1p31f) {
-                    // largest step -> [2^28, 2^29), with room for two exponents of growth
-                    const float next = pow2_field(282 - (int)(__float_as_uint(big) >> 23));
-                    const float f = next * pow2_inverse(vscale);
-                    vscale = next;
+                return big;
+            };
+            bool over = false;
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < (MASKED ? NT : 1); nt++)
 #pragma unroll
-                        for (int ng = 0; ng < NG; ng++)
+                for (int c = 0; c < (MASKED ? 2 : 1); c++) over = over || largest(nt, c, false) * vscale[nt][c] >= 0x1p31f;
+            if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                for (int k = 0; k < 4; k++) acc[nt][ng][i][k] *= f;
-                }
+                    for (int c = 0; c < 2; c++) {
+                        float big = largest(nt, c, true);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                        if (big * vscale[nt][c] >= 0x1p31f) {
+                            // largest step -> [2^28, 2^29), with room for two exponents of growth
+                            const float next = pow2_field(282 - (int)(__float_as_uint(big) >> 23));
+                            const float f = next * pow2_inverse(vscale[nt][c]);
+                            vscale[nt][c] = next;
+#pragma unroll
+                            for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    acc[nt][ng][i][c] *= f;
+                                    acc[nt][ng][i][c + 2] *= f;
+                                }
+                        }
+                    }
             }
             // ---- weights (FP32 statistics, FP16 operands) and out += codes_V^T . weights
             float off[NT][2];
@@ -645,18 +653,19 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int ng = 0; ng < NG; ng++) {
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
-                            const float vs = meta_step(vm[j][k][ng]) * vscale, vz = meta_low(vm[j][k][ng]);
+                            const float vs = meta_step(vm[j][k][ng]), vz = meta_low(vm[j][k][ng]);
+                            const float vt = vs * vscale[0][0];
                             float x[2];
                             if constexpr (!MASKED && Sh::kPacked) {
-                                x[0] = p[2 * k] * vs;
-                                x[1] = p[2 * k + 1] * vs;
+                                x[0] = p[2 * k] * vt;
+                                x[1] = p[2 * k + 1] * vt;
                                 fma2(az[nt][ng][0], az[nt][ng][1], p[2 * k], p[2 * k + 1], vz, vz, az[nt][ng][0], az[nt][ng][1]);
                             } else {
 #pragma unroll
                                 for (int c = 0; c < 2; c++) {
                                     // a position that this column does not see may hold NaN, and 0 * NaN is not 0
                                     const bool hidden = MASKED && S[j][nt][2 * k + c] == -INFINITY;
-                                    x[c] = hidden ? 0.0f : p[2 * k + c] * vs;
+                                    x[c] = hidden ? 0.0f : p[2 * k + c] * (MASKED ? vs * vscale[nt][c] : vt);
                                     az[nt][ng][c] = hidden ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
                                 }
                             }
@@ -715,12 +724,12 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                 if (g == 0) s_m[w * COLS + nt * 8 + 2 * t + c] = m[nt][c];
             }
         __syncthreads();
-        const float even = 16777216.0f * pow2_inverse(vscale), odd = 1048576.0f * pow2_inverse(vscale);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int col = nt * 8 + 2 * t + c;
+                const float even = 16777216.0f * pow2_inverse(vscale[nt][c]), odd = 0.0625f * even;
                 float M = s_m[col];
                 for (int k = 1; k < kPaWarps; k++) M = fmaxf(M, s_m[k * COLS + col]);
                 const float f = ex2(m[nt][c] - M);  // 1 where nothing was seen: zeros (or NaN) are joined

@@ -32,3 +32,25 @@ def test_attention_of_values_near_the_largest(cuda, NKV, ratio, hs, length):
     st = _attention_state(NKV, ratio, hs, 16, [length, 33], [2, 1], 72, q_scale=2.0)
     st[3][:, 1] = (st[3][:, 1].float() * 2.0 ** 124).to(BF)
     _check_attention(st, _attend(st, 2))
+
+
+@pytest.mark.parametrize("NKV,ratio,hs,bs", [(2, 1, 64, 16), (1, 8, 128, 32), (2, 4, 64, 16), (2, 4, 128, 64), (3, 1, 128, 16)])
+@pytest.mark.parametrize("power", [20, 24, 30, 40, 60])
+def test_attention_does_not_feel_hidden_outliers(cuda, NKV, ratio, hs, bs, power):
+    """V at a draft's own position is 2^power larger: the rows before it, which do not see it, have the same bits as
+    with nothing there; the row that sees it has its own values."""
+    lens, rows = [70, 45, 300], [5, 3, 2]
+    NH, qkv, codes, scales, table, lens, start = _attention_state(NKV, ratio, hs, bs, lens, rows, 73)
+    large, none = scales.clone(), scales.clone()
+    for b, n in enumerate(lens.tolist()):
+        at = (int(table[b, (n - 1) // bs]), 1, slice(None), (n - 1) % bs)
+        large[at] = (scales[at].float() * 2.0 ** power).to(BF)
+        none[at] = 0
+    hidden = [0, 1, 2, 3, 5, 6, 8]
+    st = (NH, qkv, codes, large, table, lens, start)
+    out = _attend(st, 5)
+    clean = (NH, qkv, codes, none, table, lens, start)
+    without = _attend(clean, 5)
+    assert torch.equal(out[hidden], without[hidden])
+    _check_attention(clean, without)
+    _check_attention(st, out)
