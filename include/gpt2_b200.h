@@ -284,7 +284,7 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
  * [0, rows] are cut and reported (GPT2B_DEVERR_BAD_POS); a block outside the cache
  * is left out and reported (GPT2B_DEVERR_BAD_BLOCK).  What a row does not see has no
  * part in its result, whatever it holds.  Scores and sums are in 32 bits; a weight times V's
- * step, which multiplies the codes, is held in FP16: off by 2^-12 of itself, or by 2^-29 of the largest V step
+ * step, which multiplies the codes, is held in FP16: off by 2^-11 of itself, or by 2^-29 of the largest V step
  * of that head that the row sees (weight 1) where that is more.  out overlaps neither qkv
  * nor the workspace.  scale: of the scores (1/sqrt(hs)), at most 1e30.  max_q: the most rows a request has, a hint for the tile choice.
  * workspace: gpt2b_attention_paged_w4_workspace() bytes for the same NH, NKV, hs,
