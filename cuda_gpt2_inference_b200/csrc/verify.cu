@@ -331,6 +331,15 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
             if (owner < 0 && upto + seg[k].sum > t) { owner = k; run = upto; }
             upto += seg[k].sum;
         }
+        if (owner < 0) {
+            // the CTA's sum, added in another order, passed t by a rounding: its last warp with weight
+            double before = upto = run;
+            for (int k = 0; k < kVerWarps; k++) {
+                if (seg[k].sum > 0.0) { owner = k; before = upto; }
+                upto += seg[k].sum;
+            }
+            run = before;
+        }
     }
     if (w != max(owner, 0)) return;
     int pick = last_all;
