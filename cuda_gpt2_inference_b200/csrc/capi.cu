@@ -36,6 +36,22 @@ int max_dyn_smem() {
     return cache[dev];
 }
 
+// The first error among these words, all of them cleared.
+template <size_t N> static int first_error(const int (&v)[N], int* code) {
+    *code = 0;
+    for (int x : v) {
+        if (x < 0) return GPT2B_ERR_CUDA;
+        if (x && !*code) *code = x;
+    }
+    return GPT2B_OK;
+}
+
+int engine_device_error(int* code) {
+    const int v[] = {gemv_device_error(), attention_device_error(), norm_device_error(), sampler_device_error(),
+                     persistent_device_error()};
+    return first_error(v, code);
+}
+
 int status_from(cudaError_t e) { return e == cudaSuccess ? GPT2B_OK : GPT2B_ERR_CUDA + (int)e; }
 
 }  // namespace gpt2b
@@ -63,15 +79,10 @@ const char* gpt2b_status_string(int s) {
 
 int gpt2b_device_error(int* code) {
     if (!code) return GPT2B_ERR_INVALID_ARG;
-    const int v[8] = {gemv_device_error(),       attention_device_error(), norm_device_error(),
-                      sampler_device_error(),    persistent_device_error(), paged_kv_device_error(),
-                      paged_attention_device_error(), verify_device_error()};
-    *code = 0;
-    for (int x : v) {
-        if (x < 0) return GPT2B_ERR_CUDA;
-        if (x && !*code) *code = x;
-    }
-    return GPT2B_OK;
+    int engine = 0;
+    if (const int rc = engine_device_error(&engine)) return rc;
+    const int v[] = {engine, paged_kv_device_error(), paged_attention_device_error(), verify_device_error()};
+    return first_error(v, code);
 }
 
 }  // extern "C"

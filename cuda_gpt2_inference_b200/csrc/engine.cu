@@ -1168,7 +1168,7 @@ int gpt2b_engine_generate(gpt2b_engine* e, const int* prompt, int n_prompt, int 
     if (err == cudaSuccess) err = cudaStreamSynchronize(st);
     if (err != cudaSuccess) return status_from(err);
     int dev = 0;
-    gpt2b_device_error(&dev);
+    engine_device_error(&dev);
     return dev ? GPT2B_ERR_DEVICE : GPT2B_OK;
 }
 
@@ -1292,7 +1292,7 @@ extern "C" int gpt2b_engine_generate_dump(gpt2b_engine* e, const int* prompt, in
     if (err != cudaSuccess) return status_from(err);
     if (rc != GPT2B_OK) return rc;
     int dev = 0;
-    gpt2b_device_error(&dev);
+    engine_device_error(&dev);
     if (dev) return GPT2B_ERR_DEVICE;
     if (dump->ppl_len > 0) {
         if (nll_out) memcpy(nll_out, nll.data(), nll.size() * sizeof(float));

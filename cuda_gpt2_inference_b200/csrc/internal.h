@@ -178,6 +178,10 @@ int paged_kv_device_error();
 int paged_attention_device_error();
 int verify_device_error();
 
+// gpt2b_device_error() of the kernels that an engine launches: what a run of the engine reports and clears.  The
+// operators for batches, which may run beside it, keep their words for the caller.
+int engine_device_error(int* code);
+
 // Chooses rows per tile / stages / grid for an M x K matrix of kind wk.
 // Returns false when the shape cannot be tiled (row larger than a tile).
 bool plan_gemv(GemvParams& p, int wk, int nsm, bool single_wave);

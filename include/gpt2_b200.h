@@ -56,7 +56,9 @@ enum {
 };
 
 const char* gpt2b_status_string(int status);
-/* Reads and clears the device error word of the current device (0 = none). */
+/* Reads and clears the device error word of the current device (0 = none).  An engine's generate and dump calls
+ * do the same for the kernels that an engine launches, and fail with GPT2B_ERR_DEVICE; errors of the operators for
+ * batches of requests stay for this call. */
 int gpt2b_device_error(int* code);
 int gpt2b_version(void);
 
