@@ -6,7 +6,9 @@ arch=compute_100a,code=sm_100a -lineinfo -O3 --use_fast_math``) into
 reference build (Makefile:137) so fast-math divisions in the quantisers give
 the reference's bytes.  Objects go to ``cuda_gpt2_inference_b200/_build/``.
 ``csrc/bind.cpp`` (operators on torch tensors without ctypes) becomes
-``cuda_gpt2_inference_b200/_bind.so``, against the headers of the installed torch.
+``cuda_gpt2_inference_b200/_bind.so``, against the headers of the installed torch, and is
+built again when torch or Python changes.  The library is linked whatever becomes of it, and it is left out,
+with a message, where torch, g++ or Python's headers are absent: C and C++ callers need none of them.
 
 Usage: ``python -m cuda_gpt2_inference_b200.build [--force] [--verbose] [--trace]``.
 ``--trace`` builds ``libgpt2b_trace.so`` instead (objects in ``_build_trace/``): the
@@ -19,8 +21,10 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.metadata
 import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -30,6 +34,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libgpt2b.so")
 BIND = os.path.join(HERE, "_bind.so")
+BIND_FOR = os.path.join(OBJ, "bind_for.txt")  # the torch and Python that _bind.so was built against
 OBJ_TRACE = os.path.join(HERE, "_build_trace")
 LIB_TRACE = os.path.join(HERE, "libgpt2b_trace.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
@@ -58,13 +63,33 @@ def _run(cmd, verbose=False):
         print(" ".join(cmd))
     p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if p.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + p.stdout[-6000:])
+        raise RuntimeError(os.path.basename(cmd[0]) + " failed:\n" + " ".join(cmd) + "\n" + p.stdout[-6000:])
     return p.stdout
 
 
 def _headers():
     return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
         glob.glob(os.path.join(INCLUDE, "*.h"))
+
+
+def _bind_missing():
+    """What keeps the binding from being built here, or None."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return "torch"
+    if not os.path.exists(os.path.join(spec.submodule_search_locations[0], "include", "ATen", "core", "Tensor.h")):
+        return "torch's headers"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    return None if shutil.which("g++") else "g++"
+
+
+def _bind_for():
+    try:
+        torch = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        torch = "?"
+    return f"torch {torch} in {importlib.util.find_spec('torch').submodule_search_locations[0]}, Python {sys.version}"
 
 
 def _bind_command():
@@ -76,9 +101,27 @@ def _bind_command():
             "-ltorch_cpu", "-lc10_cuda", "-lc10", f"-Wl,-rpath,{libs}"]
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> bool:
+    """Compile csrc/bind.cpp into _bind.so where it is out of date; False (and a message) where that cannot be done."""
+    missing = _bind_missing()
+    if missing:
+        print(f"{os.path.basename(BIND)} left out: no {missing} here; the operators for batches on torch tensors "
+              "(ops.py) need it, the C ABI does not", file=sys.stderr)
+        return False
+    made_for = open(BIND_FOR).read() if os.path.exists(BIND_FOR) else ""
+    sources = [os.path.join(CSRC, "bind.cpp"), os.path.join(INCLUDE, "gpt2_b200.h"), __file__]
+    if force or not os.path.exists(BIND) or made_for != _bind_for() or \
+            os.path.getmtime(BIND) < max(os.path.getmtime(f) for f in sources):
+        _run(_bind_command(), verbose)
+        os.makedirs(os.path.dirname(BIND_FOR), exist_ok=True)
+        with open(BIND_FOR, "w") as f:
+            f.write(_bind_for())
+    return True
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None, ptxas_info: bool = False,
           trace: bool = False) -> str:
-    """Compile csrc/*.cu into libgpt2b.so (or the trace build) incrementally and return its path."""
+    """Compile csrc/*.cu into libgpt2b.so (or the trace build) and _bind.so, incrementally; returns the library's path."""
     obj_dir, lib = (OBJ_TRACE, LIB_TRACE) if trace else (OBJ, LIB)
     os.makedirs(obj_dir, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -88,10 +131,6 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None, p
     if trace:
         extra.append("-DGPT2B_PERSIST_TRACE=1")
     objs, work = [], []
-    bind_src = os.path.join(CSRC, "bind.cpp")
-    if not trace and (force or not os.path.exists(BIND) or os.path.getmtime(BIND) < max(
-            os.path.getmtime(bind_src), os.path.getmtime(os.path.join(INCLUDE, "gpt2_b200.h")), os.path.getmtime(__file__))):
-        work.append(_bind_command())
     for s in srcs:
         o = os.path.join(obj_dir, os.path.basename(s)[:-3] + ".o")
         objs.append(o)
@@ -102,15 +141,18 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None, p
                 cmd.insert(1, "-Xptxas=-v")
             work.append(cmd)
     with cf.ThreadPoolExecutor(max_workers=jobs or os.cpu_count() or 4) as ex:
+        binding = None if trace else ex.submit(build_binding, force, verbose)
         outs = list(ex.map(lambda c: _run(c, verbose), work))
-    if ptxas_info:
-        for o in outs:
-            print(o)
-    if force or not os.path.exists(lib) or any(os.path.getmtime(lib) < os.path.getmtime(o) for o in objs):
-        link = [NVCC, *ARCH, "-shared", "-o", lib, *objs, "-lcudart"]
-        if nccl_lib:
-            link += [f"-L{nccl_lib}", "-l:libnccl.so.2", f"-Xlinker=-rpath,{nccl_lib}"]
-        _run(link, verbose)
+        if ptxas_info:
+            for o in outs:
+                print(o)
+        if force or not os.path.exists(lib) or any(os.path.getmtime(lib) < os.path.getmtime(o) for o in objs):
+            link = [NVCC, *ARCH, "-shared", "-o", lib, *objs, "-lcudart"]
+            if nccl_lib:
+                link += [f"-L{nccl_lib}", "-l:libnccl.so.2", f"-Xlinker=-rpath,{nccl_lib}"]
+            _run(link, verbose)
+        if binding:
+            binding.result()  # an error of its compiler comes after the library is there
     return lib
 
 

@@ -178,7 +178,11 @@ def _b():
     global _bind
     if _bind is None:
         dll = lib()
-        from . import _bind as module
+        try:
+            from . import _bind as module
+        except ImportError as e:
+            raise ImportError("the operators for batches need _bind.so, built against the torch and Python in use: "
+                              "build it with `python -m cuda_gpt2_inference_b200.build`") from e
         module.init(Gpt2bError, {n: ctypes.cast(getattr(dll, n), ctypes.c_void_p).value for n in
                                  ("gpt2b_kv_block_tables", "gpt2b_kv_cache_write_w4", "gpt2b_kv_cache_read_w4",
                                   "gpt2b_attention_forward_paged_w4", "gpt2b_softmax_probs", "gpt2b_verify_draft_tokens")})
