@@ -15,6 +15,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/gpt2_b200.h"
 
 namespace gpt2b {
@@ -298,6 +300,20 @@ inline cudaError_t ensure_smem_limit(Kernel k, unsigned long long* mask) {
 inline bool ranges_overlap(const void* p, size_t n, const void* q, size_t m) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
     return p && q && n && m && a < b + m && b < a + n;
+}
+struct ByteRange {
+    const void* p;
+    size_t n;
+};
+// Whether an output shares a byte with an input or with another output.
+inline bool outputs_overlap(std::initializer_list<ByteRange> out, std::initializer_list<ByteRange> in) {
+    for (const ByteRange* o = out.begin(); o != out.end(); ++o) {
+        for (const ByteRange& i : in)
+            if (ranges_overlap(o->p, o->n, i.p, i.n)) return true;
+        for (const ByteRange* x = out.begin(); x != o; ++x)
+            if (ranges_overlap(o->p, o->n, x->p, x->n)) return true;
+    }
+    return false;
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

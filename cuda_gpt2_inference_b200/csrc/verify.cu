@@ -426,9 +426,12 @@ int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* token
         return GPT2B_ERR_INVALID_ARG;
     if (rows > 0 && (!tokens || !target_probs || !u_accept)) return GPT2B_ERR_INVALID_ARG;
     if (draft_probs && ld_draft < V) return GPT2B_ERR_INVALID_ARG;
-    const size_t out_bytes = 4 * (size_t)B * max_out, b4 = 4 * (size_t)B, r4 = 4 * (size_t)rows;
-    if (ranges_overlap(out_tokens, out_bytes, tokens, r4) || ranges_overlap(out_tokens, out_bytes, row_start, b4 + 4) ||
-        ranges_overlap(n_accepted, b4, tokens, r4) || ranges_overlap(n_accepted, b4, row_start, b4 + 4))
+    // a request's results may be written before another's inputs are read
+    const size_t b4 = 4 * (size_t)B, r4 = 4 * (size_t)rows;
+    auto row_bytes = [&](int ld) { return rows > 0 ? 4 * ((size_t)(rows - 1) * ld + V) : 0; };
+    if (outputs_overlap({{out_tokens, b4 * max_out}, {n_accepted, b4}},
+                        {{tokens, r4}, {target_probs, row_bytes(ld_target)}, {draft_probs, row_bytes(ld_draft)},
+                         {row_start, b4 + 4}, {u_accept, r4}, {u_sample, b4}}))
         return GPT2B_ERR_INVALID_ARG;
     if (V > 1 << 30) return GPT2B_ERR_UNSUPPORTED;
     VerifyArgs a{out_tokens, n_accepted, tokens, target_probs, draft_probs, row_start, u_accept, u_sample,

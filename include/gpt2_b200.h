@@ -366,7 +366,7 @@ int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int 
  * out_tokens [B][max_out]: the accepted drafts, the drawn token, then -1; at most
  * max_out - 1 drafts are looked at.  n_accepted [B].  A request without rows gets
  * -1s and 0.  row_start outside [0, rows] is cut and reported
- * (GPT2B_DEVERR_BAD_POS).  The outputs overlap neither tokens nor row_start.  No
+ * (GPT2B_DEVERR_BAD_POS).  No output overlaps an input or the other output.  No
  * counterpart in the reference. */
 int gpt2b_verify_draft_tokens(int* out_tokens, int* n_accepted, const int* tokens, const float* target_probs,
                               const float* draft_probs, const int* row_start, const float* u_accept, const float* u_sample,

@@ -1,0 +1,41 @@
+"""Calls of the operators for batches that would overwrite what they read, or that the header does not allow (no GPU:
+refused before any launch)."""
+from __future__ import annotations
+
+import pytest
+
+FAR = 1 << 40
+
+
+def _addresses(names):
+    return {n: (i + 1) * FAR for i, n in enumerate(names)}  # far apart, 16-byte aligned, never read
+
+
+def _clash(call, at, ok, writes, reads, refused):
+    """Every output on every input and on every other output, as a whole and by a byte."""
+    for w in writes:
+        for r in [*reads, *[x for x in writes if x != w]]:
+            for by in (0, 16):
+                assert call({**at, w: at[r] + by}) == refused, (w, r, by)
+    assert call(at) != refused and ok(call(at))
+
+
+def _not_refused(gpt2b):
+    # without a GPU the launch fails, with one nothing may be launched on these addresses: only the CPU run calls it
+    return lambda rc: rc >= gpt2b.ERR_CUDA
+
+
+@pytest.fixture()
+def no_gpu():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("calls with made-up addresses that pass the checks")
+
+
+def test_verify_outputs_over_inputs(gpt2b, no_gpu):
+    names = ["out", "n", "tokens", "p", "q", "start", "ua", "us"]
+
+    def call(a):
+        return gpt2b.lib().gpt2b_verify_draft_tokens(*[a[n] for n in names], 8, 16, 100, 128, 128, 6, None)
+
+    _clash(call, _addresses(names), _not_refused(gpt2b), ["out", "n"], names[2:], gpt2b.ERR_INVALID_ARG)
