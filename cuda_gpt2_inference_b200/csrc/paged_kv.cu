@@ -333,13 +333,10 @@ int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions,
     if (B > kTableMaxRequests || (long long)max_blocks * block_size > INT_MAX) return GPT2B_ERR_UNSUPPORTED;
     // every CTA reads the inputs while others write
     const size_t b4 = 4 * (size_t)B, r = (size_t)max_rows;
-    const struct { const void* p; size_t n; } in[] = {{ctx_lens, b4}, {new_lens, b4}, {blocks_have, b4},
-                                                      {free_list, 4 * (size_t)free_cap}, {free_count, 4}},
-                                              out[] = {{block_table, b4 * max_blocks}, {slot_map, 8 * r}, {positions, 4 * r},
-                                                       {row_start, b4 + 4}, {seq_lens, b4}, {blocks_out, b4}, {free_left, 4}};
-    for (const auto& o : out)
-        for (const auto& i : in)
-            if (ranges_overlap(o.p, o.n, i.p, i.n)) return GPT2B_ERR_INVALID_ARG;
+    if (outputs_overlap({{block_table, b4 * max_blocks}, {slot_map, 8 * r}, {positions, 4 * r}, {row_start, b4 + 4},
+                         {seq_lens, b4}, {blocks_out, b4}, {free_left, 4}},
+                        {{ctx_lens, b4}, {new_lens, b4}, {blocks_have, b4}, {free_list, 4 * (size_t)free_cap}, {free_count, 4}}))
+        return GPT2B_ERR_INVALID_ARG;
     TableArgs a{block_table, slot_map, positions, row_start, seq_lens, blocks_out, free_left, ctx_lens, new_lens,
                 blocks_have, free_list, free_count, B, max_blocks, block_size, max_rows, free_cap};
     static unsigned long long mask = 0;  // 4096 requests take 48 KB

@@ -262,7 +262,8 @@ int gpt2b_attention_forward_kv_large_bf16_noalloc(uint16_t* out, const uint16_t*
  *                     that is not served and behind the last request
  * and changes nothing else, so the same call again gives the same result; the
  * caller takes blocks_out and *free_left over as the next step's blocks_have and
- * *free_count.  No output may overlap an input (GPT2B_ERR_INVALID_ARG).  free_cap is the length of free_list.  B <= 4096. */
+ * *free_count.  No output may overlap an input or another output
+ * (GPT2B_ERR_INVALID_ARG).  free_cap is the length of free_list.  B <= 4096. */
 int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions, int* row_start, int* seq_lens,
                           int* blocks_out, int* free_left, const int* ctx_lens, const int* new_lens,
                           const int* blocks_have, const int* free_list, const int* free_count, int B, int max_blocks,

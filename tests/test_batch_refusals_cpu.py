@@ -39,3 +39,18 @@ def test_verify_outputs_over_inputs(gpt2b, no_gpu):
         return gpt2b.lib().gpt2b_verify_draft_tokens(*[a[n] for n in names], 8, 16, 100, 128, 128, 6, None)
 
     _clash(call, _addresses(names), _not_refused(gpt2b), ["out", "n"], names[2:], gpt2b.ERR_INVALID_ARG)
+
+
+def test_table_outputs_over_each_other(gpt2b, no_gpu):
+    names = ["table", "slots", "positions", "start", "lens", "blocks", "left", "ctx", "new", "have", "free", "count"]
+
+    def call(a):
+        return gpt2b.lib().gpt2b_kv_block_tables(*[a[n] for n in names], 8, 16, 16, 100, 64, None)
+
+    # by a byte range: `left` and `count` are 4 bytes, so only the same address clashes with them
+    at = _addresses(names)
+    for w in names[:7]:
+        for r in names:
+            if r != w:
+                assert call({**at, w: at[r]}) == gpt2b.ERR_INVALID_ARG, (w, r)
+    assert _not_refused(gpt2b)(call(at))
