@@ -908,10 +908,6 @@ int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const u
     if (rc) return rc;
     if (workspace_bytes < need || ((long long)NH + 2ll * NKV) * hs > ld) return GPT2B_ERR_INVALID_ARG;
     if (!(scale >= -1e30f && scale <= 1e30f)) return GPT2B_ERR_INVALID_ARG;
-    const size_t out_bytes = (size_t)rows * NH * hs * 2;
-    if (rows > 0 && (ranges_overlap(out, out_bytes, qkv, ((size_t)(rows - 1) * ld + (size_t)(NH + 2 * NKV) * hs) * 2) ||
-                     ranges_overlap(workspace, need, out, out_bytes)))
-        return GPT2B_ERR_INVALID_ARG;
     // (positions are counted a few units past the end in 32 bits)
     if (block_size % kW4Tile != 0 || B > kTableMaxRequests || (long long)max_blocks * block_size > 1 << 30)
         return GPT2B_ERR_UNSUPPORTED;
@@ -921,6 +917,11 @@ int gpt2b_attention_forward_paged_w4(uint16_t* out, const uint16_t* qkv, const u
     if (rows == 0) return GPT2B_OK;
     if ((long long)rows * NH > INT_MAX - 64) return GPT2B_ERR_UNSUPPORTED;
     if ((long long)NKV * block_size * hs > INT_MAX) return GPT2B_ERR_UNSUPPORTED;  // bytes of a block
+    const size_t codes = (size_t)NKV * block_size * hs * num_blocks, b4 = 4 * (size_t)B;
+    if (outputs_overlap({{out, 2 * (size_t)rows * NH * hs}, {workspace, need}},
+                        {{qkv, 2 * ((size_t)(rows - 1) * ld + ((size_t)NH + 2 * (size_t)NKV) * hs)}, {kv_cache, codes},
+                         {kv_scale, codes / 8}, {block_table, b4 * max_blocks}, {seq_lens, b4}, {row_start, b4 + 4}}))
+        return GPT2B_ERR_INVALID_ARG;
     const PagedAttnArgs a{(__nv_bfloat16*)out, (const __nv_bfloat16*)qkv, kv_cache, (const uint32_t*)kv_scale, block_table,
                           seq_lens, row_start, B, rows, NH, NKV, ld, num_blocks, block_size, max_blocks,
                           kPaUnit / block_size, kPaUnit % block_size,

@@ -361,6 +361,11 @@ static bool w4_too_large(int NKV, int hs, int num_blocks, int block_size) {
     return block > INT_MAX || block / (kW4Group / 2) * num_blocks >= (long long)kNoRow;
 }
 
+// bytes of a cache's codes; its steps take an eighth
+static size_t w4_code_bytes(int NKV, int hs, int num_blocks, int block_size) {
+    return (size_t)NKV * block_size * hs * num_blocks;
+}
+
 int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_t* qkv, const long long* slot_map, int rows,
                             int NH, int NKV, int hs, int ld, int num_blocks, int block_size, gpt2b_stream_t stream) {
     int rc = w4_check(kv_cache, kv_scale, NKV, hs, num_blocks, block_size);
@@ -370,6 +375,10 @@ int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_
     if (w4_too_large(NKV, hs, num_blocks, block_size)) return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(qkv) || ld % 8 != 0) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
+    const size_t bytes = w4_code_bytes(NKV, hs, num_blocks, block_size);
+    if (outputs_overlap({{kv_cache, bytes}, {kv_scale, bytes / 8}},
+                        {{qkv, 2 * ((size_t)(rows - 1) * ld + ((size_t)NH + 2 * (size_t)NKV) * hs)}, {slot_map, 8 * (size_t)rows}}))
+        return GPT2B_ERR_INVALID_ARG;
     const RowGrid g = row_grid(rows, NKV, hs, kWriteChannels, kWriteAhead);
     return status_from(launch_k(kv_write_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, true, kv_cache,
                                 (uint32_t*)kv_scale, (const __nv_bfloat16*)qkv, slot_map, rows, NH, NKV, hs, ld,
@@ -384,6 +393,10 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
     if (w4_too_large(NKV, hs, num_blocks, block_size)) return GPT2B_ERR_UNSUPPORTED;
     if (!aligned16(out)) return GPT2B_ERR_ALIGNMENT;
     if (rows == 0) return GPT2B_OK;
+    const size_t bytes = w4_code_bytes(NKV, hs, num_blocks, block_size);
+    if (outputs_overlap({{out, 4 * (size_t)rows * NKV * hs}},
+                        {{kv_cache, bytes}, {kv_scale, bytes / 8}, {slot_map, 8 * (size_t)rows}}))
+        return GPT2B_ERR_INVALID_ARG;
     const RowGrid g = row_grid(rows, NKV, hs, kReadChannels, kReadAhead);
     return status_from(launch_k(kv_read_w4_kernel, dim3(g.grid), dim3(kRwThreads), 0, (cudaStream_t)stream, true,
                                 (__nv_bfloat16*)out, kv_cache, (const uint32_t*)kv_scale, slot_map, rows, NKV, hs,

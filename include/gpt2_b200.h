@@ -273,11 +273,13 @@ int gpt2b_kv_block_tables(int* block_table, long long* slot_map, int* positions,
  * (quotients within 2^-17 of a half) to even, at most 15.  A group with a NaN or an infinity is held as NaN.  A
  * negative slot skips the row; a slot outside the cache is skipped and reported
  * (GPT2B_DEVERR_BAD_BLOCK).  The non-negative slots of a call must differ: of two
- * rows with one slot, either may be held, or a mix of their groups. */
+ * rows with one slot, either may be held, or a mix of their groups.  The cache overlaps
+ * neither qkv nor slot_map, nor its codes its steps. */
 int gpt2b_kv_cache_write_w4(uint8_t* kv_cache, uint16_t* kv_scale, const uint16_t* qkv, const long long* slot_map, int rows,
                             int NH, int NKV, int hs, int ld, int num_blocks, int block_size, gpt2b_stream_t stream);
 /* Reads rows back as BF16 values: out [rows][2 (K|V)][NKV][hs]; zeros for a
- * negative slot, and for one outside the cache, which is also reported. */
+ * negative slot, and for one outside the cache, which is also reported.  out overlaps
+ * no input. */
 int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_t* kv_scale, const long long* slot_map,
                            int rows, int NKV, int hs, int num_blocks, int block_size, gpt2b_stream_t stream);
 /* Attention of the packed rows over the cache: row i of request b's n rows sees
@@ -288,8 +290,8 @@ int gpt2b_kv_cache_read_w4(uint16_t* out, const uint8_t* kv_cache, const uint16_
  * is left out and reported (GPT2B_DEVERR_BAD_BLOCK).  What a row does not see has no
  * part in its result, whatever it holds.  Scores and sums are in 32 bits; a weight times V's
  * step, which multiplies the codes, is held in FP16: off by 2^-11 of itself, or by 2^-29 of the largest V step
- * of that head that the row sees (weight 1) where that is more.  out overlaps neither qkv
- * nor the workspace.  scale: of the scores (1/sqrt(hs)), at most 1e30.  max_q: the most rows a request has, a hint for the tile choice.
+ * of that head that the row sees (weight 1) where that is more.  Neither out nor the
+ * workspace overlaps the other or an input.  scale: of the scores (1/sqrt(hs)), at most 1e30.  max_q: the most rows a request has, a hint for the tile choice.
  * workspace: gpt2b_attention_paged_w4_workspace() bytes for the same NH, NKV, hs,
  * max_q on the current device, 16-byte aligned; needs no initialisation and holds
  * nothing between calls; calls that can overlap need one each.  B <= 4096,

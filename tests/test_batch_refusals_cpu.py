@@ -54,3 +54,27 @@ def test_table_outputs_over_each_other(gpt2b, no_gpu):
             if r != w:
                 assert call({**at, w: at[r]}) == gpt2b.ERR_INVALID_ARG, (w, r)
     assert _not_refused(gpt2b)(call(at))
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_cache_and_attention_outputs_over_inputs(gpt2b, no_gpu, rows):
+    lib = gpt2b.lib()
+
+    def write(a):
+        return lib.gpt2b_kv_cache_write_w4(a["codes"], a["scales"], a["qkv"], a["slots"], rows, 4, 2, 64, 512, 8, 16, None)
+
+    def read(a):
+        return lib.gpt2b_kv_cache_read_w4(a["out"], a["codes"], a["scales"], a["slots"], rows, 2, 64, 8, 16, None)
+
+    def attend(a):
+        return lib.gpt2b_attention_forward_paged_w4(a["out"], a["qkv"], a["codes"], a["scales"], a["table"], a["lens"], a["start"],
+                                                    8, rows, 4, 2, 64, 512, 8, 16, 16, 4, 0.125, a["ws"], 1 << 30, None)
+
+    at = _addresses(["out", "codes", "scales", "qkv", "slots", "table", "lens", "start", "ws"])
+    bad, ok = gpt2b.ERR_INVALID_ARG, _not_refused(gpt2b)
+    slots = ["slots"] if rows > 2 else []  # (8 bytes: the byte further clashes with nothing)
+    _clash(write, at, ok, ["codes", "scales"], ["qkv", *slots], bad)
+    _clash(read, at, ok, ["out"], ["codes", "scales", *slots], bad)
+    _clash(attend, at, ok, ["out", "ws"], ["qkv", "codes", "scales", "table", "lens", "start"], bad)
+    # an empty step touches nothing
+    assert lib.gpt2b_kv_cache_write_w4(FAR, FAR, FAR, FAR, 0, 4, 2, 64, 512, 8, 16, None) == gpt2b.OK
