@@ -76,10 +76,10 @@ int integer(PyObject* o, const char* name) {
     if (over || v < INT_MIN || v > INT_MAX) refuse(std::string(name) + " does not fit 32 bits");
     return (int)v;
 }
-float number(PyObject* o) {
+double number(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw PyRaised{};
-    return (float)v;
+    return v;
 }
 // elements between the rows of a 2-d tensor (its width where it has one row: the stride then says nothing)
 int pitch(const at::Tensor& t) { return size32(t.size(0) > 1 ? t.stride(0) : t.size(1), "a row pitch"); }
@@ -232,7 +232,7 @@ PyObject* attention_forward_paged_w4(PyObject*, PyObject* const* a, Py_ssize_t n
         if (qkv.size(1) < ((int64_t)NH + 2 * c.NKV) * c.hs || out.size(0) != rows || out.size(1) != (int64_t)NH * c.hs)
             refuse("qkv is [rows, >= (NH + 2 NKV) hs] and out [rows, NH hs]");
         if (lens.size(0) != B || start.size(0) != (int64_t)B + 1) refuse("seq_lens has B entries and row_start B + 1");
-        const float scale = a[10] == Py_None ? (c.hs == 64 ? 0.125f : 0.08838834764831845f) : number(a[10]);
+        const float scale = a[10] == Py_None ? (c.hs == 64 ? 0.125f : 0.08838834764831845f) : (float)number(a[10]);
         const Where w({&out, &qkv, &c.codes, &c.scales, &table, &lens, &start, &ws}, a[11]);
         return launch([&] {
             return p_gpt2b_attention_forward_paged_w4(ptr<uint16_t>(out), ptr<uint16_t>(qkv), ptr<uint8_t>(c.codes),
@@ -247,7 +247,9 @@ PyObject* softmax_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return entry("softmax_probs", 5, n, [&] {
         const at::Tensor& probs = tensor(a[0], "probs", at::kFloat, 2, true);
         const at::Tensor& logits = tensor(a[1], "logits", at::kFloat, 2, true);
-        const float T = number(a[2]);
+        const double T64 = number(a[2]);
+        const float T = (float)T64;
+        if (T == 0.0f && T64 != 0.0) refuse("temperature is 0 or at least 1e-30");  // not rounded to 0, which is greedy
         const int V = a[3] == Py_None ? dim32(logits, 1) : integer(a[3], "V");
         if (probs.size(0) != logits.size(0) || probs.size(1) < V || logits.size(1) < V)
             refuse("probs and logits have the same rows, of at least V columns");

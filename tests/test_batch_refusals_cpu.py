@@ -78,3 +78,17 @@ def test_cache_and_attention_outputs_over_inputs(gpt2b, no_gpu, rows):
     _clash(attend, at, ok, ["out", "ws"], ["qkv", "codes", "scales", "table", "lens", "start"], bad)
     # an empty step touches nothing
     assert lib.gpt2b_kv_cache_write_w4(FAR, FAR, FAR, FAR, 0, 4, 2, 64, 512, 8, 16, None) == gpt2b.OK
+
+
+def test_temperature_that_32_bits_hold_as_zero(gpt2b):
+    """0 asks for the largest logit; a positive temperature below FP32's range is refused, not taken for it."""
+    import torch
+
+    from cuda_gpt2_inference_b200 import ops
+    x = torch.zeros(2, 9)
+    for T in (1e-46, 1e-300, -1e-60):
+        with pytest.raises(gpt2b.Gpt2bError, match="temperature") as e:
+            ops.softmax_probs(x, x.clone(), T)
+        assert e.value.status == gpt2b.ERR_INVALID_ARG
+    with pytest.raises(gpt2b.Gpt2bError, match="CUDA"):  # what is allowed comes as far as the tensors' device
+        ops.softmax_probs(x, x.clone(), 0.0)
