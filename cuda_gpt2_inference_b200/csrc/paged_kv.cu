@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kRwThreads)
                 for (int o = 2; o > 0; o >>= 1) e = bf16x2_min_nan(e, __shfl_xor_sync(eight, e, o));
                 uint32_t meta;
                 *reinterpret_cast<uint2*>(my_codes + (size_t)at[k] * (kW4Group / 2)) =
-                    w4_encode16(u, bf16lo(e), -bf16hi(e), meta);
+                    w4_encode16(u, bf16lo(e), bf16hi(e), meta);
                 if (first) my_scales[at[k]] = meta;
             }
         }

@@ -54,3 +54,51 @@ def test_attention_does_not_feel_hidden_outliers(cuda, NKV, ratio, hs, bs, power
     assert torch.equal(out[hidden], without[hidden])
     _check_attention(clean, without)
     _check_attention(st, out)
+
+
+def _append(x, hs):
+    """x [rows, 2 NKV hs] appended to a fresh cache, one row a slot: (codes, scales) [rows, 2, NKV, ...]."""
+    from cuda_gpt2_inference_b200 import ops
+    rows, NKV = x.shape[0], x.shape[1] // (2 * hs)
+    nb = -(-rows // 16)
+    codes = torch.zeros(nb, 2, NKV, 16, hs // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(nb, 2, NKV, 16, hs // 64, 2, dtype=BF, device="cuda")
+    qkv = torch.cat([torch.zeros(rows, NKV * hs, dtype=BF), x], 1).cuda()
+    ops.kv_cache_write_w4(codes, scales, qkv, torch.arange(rows, device="cuda"), NKV)
+    return [t.cpu().transpose(2, 3).transpose(1, 2).flatten(0, 1)[:rows] for t in (codes, scales)]
+
+
+def _check_codes(x, hs, codes, scales):
+    """Steps and low ends as defined, to the bit; a code differs from its 64-bit form only where the quotient is near
+    a half: within 2^-17 (those are ties) and what its arithmetic is off by, 2^-18 (a reciprocal of 2 units in the
+    last place at most, 2^-22 of a quotient below 15.5)."""
+    want_c, want_s = plain.quantise(x.view(x.shape[0], 2, -1, hs))
+    assert torch.equal(scales.view(torch.int16), want_s.view(torch.int16))
+    g = x.view(x.shape[0], 2, -1, hs // 64, 64).double()
+    step, low = want_s[..., 0:1].double(), want_s[..., 1:2].double()
+    q = torch.where(step > 0, (g - low) / step, torch.zeros_like(g)).clamp(0, 15)
+    got, want = (torch.stack([c & 15, c >> 4], -1).flatten(-2).view(g.shape).double() for c in (codes, want_c))
+    near = (q - q.floor() - 0.5).abs() <= 2.0 ** -17 + 2.0 ** -18
+    assert ((got == want) | near).all()
+    assert ((got - q).abs() <= 0.5 + 2.0 ** -17 + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("power", [0, -60, -112, 100])
+@pytest.mark.parametrize("offset", [0.0, 3.0, 100.0])
+def test_codes_differ_only_at_ties(cuda, hs, power, offset):
+    x = ((torch.randn(500, 4 * hs, generator=torch.Generator().manual_seed(hs)) + offset) * 2.0 ** power).to(BF)
+    _check_codes(x, hs, *_append(x, hs))
+
+
+def test_append_of_subnormal_values(cuda):
+    """BF16 subnormals count: beside a step of 2^-119 they decide a quotient's half, and as an end of their group the step."""
+    g = torch.Generator().manual_seed(5)
+    tiny = torch.randint(-127, 128, (300, 128), generator=g) * 2.0 ** -133
+    x = tiny.clone()
+    x[:, 0::64], x[:, 1::64] = -15 * 2.0 ** -120, 15 * 2.0 ** -120  # quotients of the others: 7.5 +- up to 2^-7
+    x = x.to(BF)
+    _check_codes(x, 64, *_append(x, 64))
+    low = -(1 + torch.rand(300, 128, generator=g)) * 2.0 ** -116
+    x = torch.where(torch.arange(128) % 64 < 40, low, tiny).to(BF)  # the largest of a group is subnormal
+    _check_codes(x, 64, *_append(x, 64))
