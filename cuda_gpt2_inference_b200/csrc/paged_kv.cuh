@@ -80,7 +80,7 @@ __device__ __forceinline__ uint2 w4_encode16(const uint32_t* u, float lo, float 
     return make_uint2(word[0], word[1]);
 }
 
-// The 8 channels of a word as FP32: code * step + low end, one rounding.  Nibble k of a half, masked in place
+// The 8 channels of a word as FP32: code * step + low end, one rounding (subnormals kept).  Nibble k of a half, masked in place
 // under the exponent of 2^23, reads 2^23 + code * 16^k; one exact multiply-add leaves the code.
 __device__ __forceinline__ void w4_values(uint32_t word, uint32_t meta, float* x) {
     const float s = __uint_as_float(meta << 16), lo = __uint_as_float(meta & 0xffff0000u);
@@ -89,7 +89,7 @@ __device__ __forceinline__ void w4_values(uint32_t word, uint32_t meta, float* x
     for (int k = 0; k < 8; k++) {
         const uint32_t h = k < 4 ? word : word >> 16;
         const float f = __uint_as_float((h & (15u << (4 * (k & 3)))) | 0x4b000000u);
-        x[k] = fmaf(fmaf(f, down[k & 3], -8388608.0f * down[k & 3]), s, lo);
+        x[k] = fma_sub(fmaf(f, down[k & 3], -8388608.0f * down[k & 3]), s, lo);
     }
 }
 

@@ -102,3 +102,20 @@ def test_append_of_subnormal_values(cuda):
     low = -(1 + torch.rand(300, 128, generator=g)) * 2.0 ** -116
     x = torch.where(torch.arange(128) % 64 < 40, low, tiny).to(BF)  # the largest of a group is subnormal
     _check_codes(x, 64, *_append(x, 64))
+
+
+@pytest.mark.parametrize("power", [-119, -125, -130, -133])
+def test_read_back_of_subnormal_values(cuda, power):
+    """Values of a flat group, and low ends below a step, are read back as they are held."""
+    from cuda_gpt2_inference_b200 import ops
+    g = torch.Generator().manual_seed(6)
+    codes = torch.randint(0, 256, (2, 2, 1, 16, 32), generator=g, dtype=torch.uint8)
+    scales = torch.zeros(2, 2, 1, 16, 1, 2)
+    scales[..., 1] = torch.randint(-127, 128, scales.shape[:-1], generator=g) * 2.0 ** power
+    scales[1, ..., 0] = 2.0 ** -120
+    scales = scales.to(BF)
+    out = torch.zeros(32, 2, 1, 64, dtype=BF, device="cuda")
+    ops.kv_cache_read_w4(out, codes.cuda(), scales.cuda(), torch.arange(32, device="cuda"))
+    want = plain.values(codes, scales).transpose(2, 3).transpose(1, 2).flatten(0, 1)
+    # one rounding in 32 bits and one in BF16, of a value or of the smallest subnormals
+    assert ((out.cpu().double() - want).abs() <= plain.BF16 * (1 + 2.0 ** -15) * want.abs() + 2.0 ** -134 + 2.0 ** -149).all()
