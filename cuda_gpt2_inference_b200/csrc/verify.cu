@@ -199,6 +199,13 @@ struct VerifyArgs {
     int B, rows, V, ld_p, ld_q, max_out;
 };
 
+// FP32 to 64 bits with subnormals, which the build's fast arithmetic takes as 0: they are weights like others.
+__device__ __forceinline__ double widen(float x) {
+    double r;
+    asm("cvt.f64.f32 %0, %1;" : "=d"(r) : "f"(x));
+    return r;
+}
+
 constexpr int kVerThreads = 512, kVerWarps = kVerThreads / 32;
 
 // Weight of token k: 0 unless positive, so NaN counts as nothing.
@@ -206,8 +213,8 @@ struct Weights {
     const float *p, *q;
     int drop;
     __device__ __forceinline__ double operator()(int k) const {
-        double v = (double)p[k];
-        if (q) v -= (double)q[k];
+        double v = widen(p[k]);
+        if (q) v -= widen(q[k]);
         return v > 0.0 && k != drop ? v : 0.0;
     }
 };
@@ -251,8 +258,8 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
         const int i = i0 + lane, d = i < n ? a.tokens[r0 + i + 1] : -1;
         bool ok = i >= n;
         if (d >= 0 && d < a.V) {
-            const double q = a.q ? (double)a.q[(size_t)(r0 + i) * a.ld_q + d] : 1.0;
-            ok = (double)a.u_accept[r0 + i] * q < (double)a.p[(size_t)(r0 + i) * a.ld_p + d];
+            const double q = a.q ? widen(a.q[(size_t)(r0 + i) * a.ld_q + d]) : 1.0;
+            ok = widen(a.u_accept[r0 + i]) * q < widen(a.p[(size_t)(r0 + i) * a.ld_p + d]);
         }
         const unsigned no = __ballot_sync(0xffffffffu, !ok);
         if (no) {
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
 #pragma unroll
             for (int j = 0; j < kAhead; j++) {
                 const int k = k0 + 32 * j;
-                const double v = (double)p[j] - (double)q[j];
+                const double v = widen(p[j]) - widen(q[j]);
                 if (v > 0.0 && k != wt.drop) {
                     sum += v;
                     last = k;
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
     }
     // The CTA and then the warp in whose part the cumulative weight passes t, the same in every warp.  Where none
     // does (t at or beyond the total, or NaN) the last token of positive weight is drawn, by the first warp.
-    const double t = (double)u * total;
+    const double t = widen(u) * total;
     int cta = -1, owner = -1, last_all = -1;
     double upto = 0.0, run = 0.0;
     for (int k = 0; k < C; k++) {

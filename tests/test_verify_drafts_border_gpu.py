@@ -6,6 +6,7 @@ from fractions import Fraction
 import pytest
 import torch
 
+import paged_w4_plain as plain
 from test_verify_drafts_gpu import _run
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +32,22 @@ def test_draw_at_a_border_that_rounding_moves(cuda, tiny, every):
     slack = total * n / 2 ** 53 if every == 1 else total * 64 / 2 ** 53
     assert w[-1] > 0 and taken == [0]
     assert below <= total / 2 + slack and below + w[-1] >= total / 2 - slack
+
+
+@pytest.mark.parametrize("certain", [False, True])
+@pytest.mark.parametrize("u", [0.0, 0.3, 1.0, 2.0 ** -140])
+def test_subnormal_probabilities_count(cuda, certain, u):
+    """Probabilities below FP32's normal range: they are accepted against 0, are what is left of a target, and are drawn."""
+    V = 300
+    p, q = torch.zeros(8, V), torch.zeros(8, V)
+    p[0, 7] = 2.0 ** -140                         # a draft as likely as nothing else: accepted at u 0
+    p[1, 5:9] = torch.tensor([1.0, 2, 3, 4]) * 2.0 ** -149  # a row of subnormals alone
+    p[2, 40], q[2, 40] = 0.5, 0.5                 # all that is left of the target is subnormal
+    p[2, 90] = p[2, 200] = 2.0 ** -135
+    p[3, 1] = 1.0
+    p[4, 11], q[4, 11] = 2.0 ** -130, 2.0 ** -131
+    p[5, 250] = 2.0 ** -127
+    p[6, 0] = p[6, 299] = 2.0 ** -128
+    tokens = torch.tensor([0, 7, 0, 40, 0, 11, 0, 0])
+    args = (tokens, p, None if certain else q, [0, 2, 4, 6, 7], torch.full((8,), u), torch.full((4,), u), 3)
+    assert _run(*args) == plain.verify(*args)
