@@ -147,12 +147,19 @@ struct FirstMax {
     float m;
     int at;
 };
+// a > b where the build's fast comparison takes subnormals as 0
+__device__ __forceinline__ bool above(float a, float b) {
+    int r;
+    asm("{\n\t.reg .pred p;\n\tsetp.gt.f32 p, %1, %2;\n\tselp.s32 %0, 1, 0, p;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+// whether b comes before a: larger, or as large and earlier (neither is NaN)
+__device__ __forceinline__ bool before(FirstMax a, FirstMax b) { return above(b.m, a.m) || (!above(a.m, b.m) && b.at < a.at); }
 __device__ __forceinline__ FirstMax first_max(FirstMax a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        const int at = __shfl_xor_sync(0xffffffffu, a.at, o);
-        if (m > a.m || (m == a.m && at < a.at)) a = {m, at};
+        const FirstMax b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.at, o)};
+        if (before(a, b)) a = b;
     }
     return a;
 }
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(kProbThreads)
 #pragma unroll 8
     for (int i = lo + tid; i < hi; i += kProbThreads) {
         const float y = x[i];
-        if (y > a.m) a = {y, i};
+        if (above(y, a.m)) a = {y, i};
     }
     a = first_max(a);
     cluster_wait();
@@ -182,7 +189,7 @@ __global__ void __launch_bounds__(kProbThreads)
     cluster_wait();
     a = {-INFINITY, INT_MAX};
     for (int k = lane; k < C * kProbWarps; k += 32)
-        if (all[k].m > a.m || (all[k].m == a.m && all[k].at < a.at)) a = all[k];
+        if (before(a, all[k])) a = all[k];
     a = first_max(a);
     for (int i = lo + tid; i < hi; i += kProbThreads) out[i] = i == a.at ? 1.0f : 0.0f;
 }

@@ -51,3 +51,18 @@ def test_subnormal_probabilities_count(cuda, certain, u):
     tokens = torch.tensor([0, 7, 0, 40, 0, 11, 0, 0])
     args = (tokens, p, None if certain else q, [0, 2, 4, 6, 7], torch.full((8,), u), torch.full((4,), u), 3)
     assert _run(*args) == plain.verify(*args)
+
+
+@pytest.mark.parametrize("rows,V", [(1, 40), (3, 50257)])
+def test_greedy_among_subnormal_logits(cuda, rows, V):
+    """Logits that differ by a subnormal are no tie."""
+    from cuda_gpt2_inference_b200 import ops
+    x = torch.zeros(rows, V)
+    x[:, V // 3], x[:, V // 2], x[:, V - 2] = 2.0 ** -149, 3 * 2.0 ** -149, 3 * 2.0 ** -149
+    x[0] -= 0.0
+    x[-1, 5] = -(2.0 ** -140)
+    out = torch.full((rows, V), -7.0, device="cuda")
+    ops.softmax_probs(out, x.cuda(), 0.0)
+    want = torch.zeros(rows, V)
+    want[:, V // 2] = 1
+    assert torch.equal(out.cpu(), want)
