@@ -367,7 +367,8 @@ int gpt2b_softmax_probs(float* probs, const float* logits, int rows, int V, int 
  * weight.  Products, weights and sums are in 64 bits.  A draft outside [0, V) ends
  * the drafts: the token is drawn from that row's target_probs, as if it were last.
  * out_tokens [B][max_out]: the accepted drafts, the drawn token, then -1; at most
- * max_out - 1 drafts are looked at.  n_accepted [B].  A request without rows gets
+ * max_out - 1 drafts are looked at.  n_accepted [B].  Only row_start says what a request is: the results of one
+ * that kv_block_tables did not serve (seq_lens 0), or whose rows are a piece of a prompt, are to be ignored.  A request without rows gets
  * -1s and 0.  row_start outside [0, rows] is cut and reported
  * (GPT2B_DEVERR_BAD_POS).  No output overlaps an input or the other output.  No
  * counterpart in the reference. */
