@@ -568,7 +568,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                         float x = top[nt][c];
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                        const float mn = fmaxf(m[nt][c], x);
+                        // a column's own scores decide, so that its bits do not depend on another's
+                        const float mn = x > m[nt][c] + 8.0f ? x : m[nt][c];
                         const float f = mn == m[nt][c] ? 1.0f : ex2(m[nt][c] - mn);
                         m[nt][c] = mn;
                         l[nt][c] *= f;

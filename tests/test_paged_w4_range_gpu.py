@@ -119,3 +119,26 @@ def test_read_back_of_subnormal_values(cuda, power):
     want = plain.values(codes, scales).transpose(2, 3).transpose(1, 2).flatten(0, 1)
     # one rounding in 32 bits and one in BF16, of a value or of the smallest subnormals
     assert ((out.cpu().double() - want).abs() <= plain.BF16 * (1 + 2.0 ** -15) * want.abs() + 2.0 ** -134 + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("NKV,ratio,hs,bs", [(2, 1, 64, 16), (1, 8, 128, 32), (2, 4, 64, 16), (2, 4, 128, 64), (3, 1, 128, 16)])
+@pytest.mark.parametrize("factor", [0.0, 5.0, 100.0, -1e6])
+@pytest.mark.parametrize("lens,rows", [([70, 45, 300, 33], [5, 3, 4, 3]), (list(range(290, 322)), [4] * 32)])
+def test_attention_rows_do_not_depend_on_later_drafts(cuda, monkeypatch, NKV, ratio, hs, bs, factor, lens, rows):
+    """Keys and values at the last two drafts' own positions change: the rows before them keep their bits."""
+    values = plain.values
+
+    def with_negative_steps(codes, scales, magnitude=False):  # (what bounds the errors is |code * step| + |low end|)
+        return values(codes, torch.stack([scales[..., 0].abs(), scales[..., 1]], -1) if magnitude else scales, magnitude)
+
+    monkeypatch.setattr(plain, "values", with_negative_steps)
+    NH, qkv, codes, scales, table, lens, start = _attention_state(NKV, ratio, hs, bs, lens, rows, 74)
+    other = scales.clone()
+    for b, n in enumerate(lens.tolist()):
+        for p in (n - 1, n - 2):
+            at = (int(table[b, p // bs]), slice(None), slice(None), p % bs)
+            other[at] = (scales[at].float() * factor).to(BF)
+    outs = [_attend((NH, qkv, codes, s, table, lens, start), 5) for s in (scales, other)]
+    before = torch.cat([torch.arange(int(start[b]), int(start[b + 1]) - 2) for b in range(len(rows))])
+    assert torch.equal(outs[0][before], outs[1][before])
+    _check_attention((NH, qkv, codes, other, table, lens, start), outs[1])
