@@ -21,12 +21,18 @@
 // there again; here a tile has 1..16 columns, and the codes go from a register to
 // the tensor core that multiplies them.
 //
-// What bounds it: instruction issue.  A step of 32 positions of 128 channels takes a warp
-// about 540 instructions, half of them on the ALU pipe (decode, steps, maxima), which the
-// SM issues at 55 % of its rate; HBM would need 63 % of the time.  Measured, of the 6.54 TB/s
-// of a copy: 32 x 16384 positions of 8 heads of 128, one row of 4 query heads each: 125 us,
-// 74 %; 16 columns: 175 us, 53 %; 32 x 8192 of 25 heads of 64, one row: 105 us, 69 %.  One
-// request of 1001 positions and 12 heads: 6 us, a chain of launch, lengths, table, codes, join.
+// What bounds it: the latency of a warp's own arithmetic.  A step of 32 positions of 128
+// channels takes a warp about 540 instructions, half of them on the ALU pipe (decode, steps,
+// maxima).  Registers leave 3 warps a scheduler with 8 columns and 2 with 16, which issue in
+// 55 and 52 % of the cycles and wait longest for results of their own instructions; nothing is
+// full (ALU 54 and 42 %, tensor pipe 26 and 39 %).  Measured, of the 6.54 TB/s of a copy:
+// 32 x 16384 positions of 8 heads of 128, one row of 4 query heads each: 125 us, 74 %; 4 rows,
+// 16 columns: 176 us, 53 %; 32 x 8192 of 25 heads of 64, one row: 105 us, 69 %.  One request of
+// 1001 positions and 12 heads: 6 us, a chain of launch, lengths, table, codes, join.
+//
+// Weights times V's steps are the products' other operand, in FP16: 2^-11 of each, where BF16 would
+// be 2^-8 and FP32 operands have no such product.  Against 64 bits the result is off by 1.71e-3 to
+// 1.77e-3 (root mean square, relative), a 32-bit form rounded once to BF16 by 1.66e-3 to 1.68e-3.
 #include "paged_kv.cuh"
 #include "internal.h"
 
@@ -787,6 +793,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_join_kernel(PagedAttnAr
     extern __shared__ __align__(16) unsigned char smem[];
     long long* pre = reinterpret_cast<long long*>(smem);
     __shared__ long long wsum[kPaWarps];
+    // Lengths and offsets are read ahead of pdl_wait: the main launch lets this one start only behind its own wait,
+    // when whatever wrote them has ended, and does not write them itself.
     pa_scan(a, COLS, pre, wsum, false);
     const long long total = pre[a.B];
     const int G = (int)min((long long)main_grid, total), i0 = blockIdx.x;

@@ -159,7 +159,10 @@ __global__ void __launch_bounds__(kTabThreads) block_tables_kernel(TableArgs a) 
 // left gaps, 24 us against 19).  A CTA's threads cover whole rows, so a thread's head and channels are worked out
 // once.  The 8 lanes that share a row (at least) work out the places of their next 8 rows together, one each, and
 // hand them round as numbers of 32-byte groups of codes (a step to each, in the same order).  Several rows' loads
-// are in flight.  16384 rows of 2 * 8 * 128: 22 us to append and 19 to read back, of 13 each that HBM takes.
+// are in flight.  16384 rows of 2 * 8 * 128: 22 us to append and 19 to read back, of 13 each that HBM takes.  Neither
+// is full of anything (issue slots 69 and 68 %, ALU pipe 45 and 57 %): with 7 warps a scheduler the batches of loads
+// that a thread works through one behind the other, the places of the next rows among them, are most of the wait
+// (4.0 and 3.8 of 10.2 cycles an instruction).
 constexpr int kRwThreads = 256, kWriteChannels = 16, kReadChannels = 8, kWriteAhead = 2, kReadAhead = 4;
 constexpr uint32_t kNoRow = 0xffffffffu;
 
@@ -189,7 +192,7 @@ __device__ __forceinline__ uint32_t slot_group(long long slot, long long slots, 
     return b * page + ((unsigned)slot - b * (unsigned)block_size) * per_pos;
 }
 
-// Bound by HBM for many rows (rows * 2 * NKV * hs * 2.56 bytes), by its launch for few.
+// Bound by the latencies above for many rows (HBM: rows * 2 * NKV * hs * 2.56 bytes), by its launch for few.
 __global__ void __launch_bounds__(kRwThreads)
     kv_write_w4_kernel(uint8_t* codes, uint32_t* scales, const __nv_bfloat16* qkv, const long long* slot_map, int rows,
                        int NH, int NKV, int hs, int ld, long long slots, int block_size, int parts, int rows_per_cta) {

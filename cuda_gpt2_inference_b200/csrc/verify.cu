@@ -2,7 +2,8 @@
 //
 // Both work on rows of a vocabulary (50257 logits: 200 KB) of which there are few: one to a
 // few hundred.  A row is therefore spread over a cluster of CTAs that exchange their partial
-// results through distributed shared memory: one launch, each row read once, no atomics.
+// results through distributed shared memory: one launch, each row read from HBM once (and a second time from L1 or L2
+// where a result needs the whole row first), no atomics.
 #include "common.cuh"
 #include "internal.h"
 
@@ -96,7 +97,8 @@ __global__ void __launch_bounds__(T, T == 256 ? 6 : 2)
 
     pdl_wait();
     // NaN goes through the maximum.  In the sum a single product serves as exponent: its error grows with the
-    // distance from the maximum, but the terms fall faster (2^-22 of the sum at a spread of 10).
+    // distance from the maximum, but the terms fall faster (2^-22 of the sum at a spread of 10; against 64 bits the
+    // result is off by 1.1e-7 on 5 rows of 50257, a plain 32-bit form by 0.6e-7).
     float v[U], m = -INFINITY, s = 0.0f;
     for (int i = 0; i < left; i += U * T) {
         float top = m;
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(T, T == 256 ? 6 : 2)
     }
 }
 
-// Temperature 0: 1 at the first largest, NaN left out.
+// Temperature 0: 1 at the first largest, NaN left out.  320 x 50257: 43 us, 5 rows 3.8 us.
 struct FirstMax {
     float m;
     int at;
@@ -237,8 +239,8 @@ struct VerPart {
 // barrier; every warp then knows in whose piece the cumulative weight passes u * total, and that warp scans its
 // piece again (from L1) and writes the request's results.  64-bit sums: with 32 bits the border of one token in
 // 200 of a 50257-token vocabulary would be off by more than a random number's own step.
-// Bound by the chain launch - offsets - drafts - row - exchange - scan: 7 us for one request of a 50257-token
-// vocabulary, 11 us for 64, whose two rows each (26 MB) take HBM 4 us.
+// Bound by the chain launch - offsets - drafts - row - exchange - scan: 6.7 us for one request of a 50257-token
+// vocabulary, 9.9 us for 64, whose two rows each (26 MB) take HBM 4 us.
 __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(VerifyArgs a) {
     __shared__ VerPart all[2][8], seg[kVerWarps];
     cluster_begin();
