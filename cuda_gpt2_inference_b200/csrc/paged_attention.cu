@@ -545,7 +545,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                         }
                     }
             }
-            if constexpr (MASKED) {  // positions that a column does not see
+            uint32_t hidden = 0;  // a bit a score: positions that a column does not see
+            if constexpr (MASKED) {
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -553,7 +554,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int p = p0 + 16 * j + tile_pos(g) + (k >> 1) * 8;
-                            if (p > lim[nt][k & 1] || ((badbits >> j) & 1u)) S[j][nt][k] = -INFINITY;
+                            if (p > lim[nt][k & 1] || ((badbits >> j) & 1u)) {
+                                S[j][nt][k] = -INFINITY;
+                                hidden |= 1u << ((j * NT + nt) * 4 + k);
+                            }
                         }
             }
             // ---- running maximum: raised only where a score passes it by 2^8, so weights stay below 2^8
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                         for (int ng = 0; ng < NG; ng++) {
                             const float x = fabsf(meta_step(vm[j][k][ng]));
-                            if ((!MASKED || S[j][nt][2 * k + c] != -INFINITY) && (!finite || x < INFINITY)) big = fmaxf(big, x);
+                            if (!(hidden >> ((j * NT + nt) * 4 + 2 * k + c) & 1u) && (!finite || x < INFINITY)) big = fmaxf(big, x);
                         }
                 return big;
             };
@@ -671,9 +675,9 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
                                 for (int c = 0; c < 2; c++) {
                                     // a position that this column does not see may hold NaN, and 0 * NaN is not 0
-                                    const bool hidden = MASKED && S[j][nt][2 * k + c] == -INFINITY;
-                                    x[c] = hidden ? 0.0f : p[2 * k + c] * (MASKED ? vs * vscale[nt][c] : vt);
-                                    az[nt][ng][c] = hidden ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
+                                    const bool none = MASKED && (hidden >> ((j * NT + nt) * 4 + 2 * k + c) & 1u);
+                                    x[c] = none ? 0.0f : p[2 * k + c] * (MASKED ? vs * vscale[nt][c] : vt);
+                                    az[nt][ng][c] = none ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
                                 }
                             }
                             wb[nt][ng][k] = mov_trans(f16x2(x[0], x[1]));

@@ -142,3 +142,24 @@ def test_attention_rows_do_not_depend_on_later_drafts(cuda, monkeypatch, NKV, ra
     before = torch.cat([torch.arange(int(start[b]), int(start[b + 1]) - 2) for b in range(len(rows))])
     assert torch.equal(outs[0][before], outs[1][before])
     _check_attention((NH, qkv, codes, other, table, lens, start), outs[1])
+
+
+@pytest.mark.parametrize("NKV,ratio,hs", [(2, 1, 64), (1, 8, 128), (2, 4, 128)])
+@pytest.mark.parametrize("at", [0, 5, 290])
+def test_attention_of_a_key_of_minus_infinity(cuda, NKV, ratio, hs, at):
+    """A score of -infinity is a weight of 0, not a hidden position: V counts there as 0 times what it holds, in a step
+    that all rows see and in one that they do not."""
+    lens, rows = [300], [3]
+    NH, qkv, codes, scales, table, lens, start = _attention_state(NKV, ratio, hs, 16, lens, rows, 75)
+    qkv = qkv.abs()
+    place = (int(table[0, at // 16]), 0, slice(None), at % 16)
+    codes[place] = 0
+    scales[place] = torch.tensor([0.0, -math.inf]).to(BF)
+    st = (NH, qkv, codes, scales, table, lens, start)
+    out = _attend(st, 3)
+    want = plain.attention(qkv, codes, scales, table, lens, start, NH)[0]
+    err = plain.attention(qkv, codes, torch.nan_to_num(scales, neginf=0.0), table, lens, start, NH)[1]  # (no infinite bound)
+    off = (out[:3].cpu().double() - want[:3]).abs()
+    assert (off <= plain.BF16 * want[:3].abs() + 1.01 * err[:3] + 2.0 ** -126).all()
+    scales[(place[0], 1, *place[2:])] = math.nan
+    assert _attend(st, 3)[:3].isnan().all()
