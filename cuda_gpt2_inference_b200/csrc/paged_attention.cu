@@ -650,6 +650,11 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 uint32_t wb[NT][NG][2];
+                float vt[NG][2];
+#pragma unroll
+                for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) vt[ng][k] = meta_step(vm[j][k][ng]) * (MASKED ? 1.0f : vscale[0][0]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float p[4];
@@ -664,19 +669,18 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<NG, NT>::kCtas) paged_attn
                     for (int ng = 0; ng < NG; ng++) {
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
-                            const float vs = meta_step(vm[j][k][ng]), vz = meta_low(vm[j][k][ng]);
-                            const float vt = vs * vscale[0][0];
+                            const float vz = meta_low(vm[j][k][ng]);
                             float x[2];
                             if constexpr (!MASKED && Sh::kPacked) {
-                                x[0] = p[2 * k] * vt;
-                                x[1] = p[2 * k + 1] * vt;
+                                x[0] = p[2 * k] * vt[ng][k];
+                                x[1] = p[2 * k + 1] * vt[ng][k];
                                 fma2(az[nt][ng][0], az[nt][ng][1], p[2 * k], p[2 * k + 1], vz, vz, az[nt][ng][0], az[nt][ng][1]);
                             } else {
 #pragma unroll
                                 for (int c = 0; c < 2; c++) {
                                     // a position that this column does not see may hold NaN, and 0 * NaN is not 0
                                     const bool none = MASKED && (hidden >> ((j * NT + nt) * 4 + 2 * k + c) & 1u);
-                                    x[c] = none ? 0.0f : p[2 * k + c] * (MASKED ? vs * vscale[nt][c] : vt);
+                                    x[c] = none ? 0.0f : p[2 * k + c] * (MASKED ? vt[ng][k] * vscale[nt][c] : vt[ng][k]);
                                     az[nt][ng][c] = none ? az[nt][ng][c] : fmaf(p[2 * k + c], vz, az[nt][ng][c]);
                                 }
                             }
