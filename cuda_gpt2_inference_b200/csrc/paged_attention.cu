@@ -27,7 +27,7 @@
 // 55 and 52 % of the cycles and wait longest for results of their own instructions; nothing is
 // full (ALU 54 and 42 %, tensor pipe 26 and 39 %).  Measured, of the 6.54 TB/s of a copy:
 // 32 x 16384 positions of 8 heads of 128, one row of 4 query heads each: 125 us, 74 %; 4 rows,
-// 16 columns: 176 us, 53 %; 32 x 8192 of 25 heads of 64, one row: 105 us, 69 %.  One request of
+// 16 columns: 175 us, 53 %; 32 x 8192 of 25 heads of 64, one row: 105 us, 69 %.  One request of
 // 1001 positions and 12 heads: 6 us, a chain of launch, lengths, table, codes, join.
 //
 // Weights times V's steps are the products' other operand, in FP16: 2^-11 of each, where BF16 would

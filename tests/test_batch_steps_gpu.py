@@ -119,3 +119,39 @@ def test_next_lengths_of_mixed_requests(cuda, gpt2b):
     assert waited > 2 and idle > 0 and told > 10 and gpt2b.device_error() == 0
     held = [table[b, :int(have[b])].tolist() for b in range(B)]
     assert sorted(sum(held, []) + free[:int(count)].tolist()) == list(range(nb))
+
+
+def test_calls_of_two_threads_at_once(cuda):
+    """The binding lets go of the interpreter lock: two threads, a stream each, the same operators at once."""
+    import threading
+
+    from cuda_gpt2_inference_b200 import ops
+    from test_paged_w4_gpu import _attend, _attention_state
+    sts = [_attention_state(2, r, hs_, 16, [700, 33], [2, 1], 90 + r) for r, hs_ in ((1, 64), (8, 128))]
+    want = [_attend(st, 2) for st in sts]
+    x = torch.randn(5, 5000, device="cuda")
+    probs = torch.empty_like(x)
+    ops.softmax_probs(probs, x, 0.7)
+    ds = [[t.cuda() for t in st[1:]] for st in sts]
+    ws = [torch.empty(ops.attention_paged_w4_workspace(st[0], 2, st[2].shape[4] * 2, 2), dtype=torch.uint8, device="cuda") for st in sts]
+    outs = [[torch.full_like(want[k], 123.0) for _ in range(50)] for k in range(2)]
+    ps = [[torch.empty_like(x) for _ in range(50)] for _ in range(2)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            for i in range(50):
+                ops.attention_forward_paged_w4(outs[k][i], *ds[k][:3], ds[k][3], ds[k][4], ds[k][5], sts[k][0], 2, ws[k], stream=s)
+                ops.softmax_probs(ps[k][i], x, 0.7, stream=s)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed
+    for k in range(2):
+        assert all(torch.equal(o, want[k]) for o in outs[k]) and all(torch.equal(p, probs) for p in ps[k])

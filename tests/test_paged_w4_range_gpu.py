@@ -163,3 +163,10 @@ def test_attention_of_a_key_of_minus_infinity(cuda, NKV, ratio, hs, at):
     assert (off <= plain.BF16 * want[:3].abs() + 1.01 * err[:3] + 2.0 ** -126).all()
     scales[(place[0], 1, *place[2:])] = math.nan
     assert _attend(st, 3)[:3].isnan().all()
+
+
+@pytest.mark.parametrize("NKV,ratio,hs,bs", [(2, 4, 128, 32), (3, 1, 64, 16)])
+def test_attention_of_prompt_pieces(cuda, NKV, ratio, hs, bs):
+    """Hundreds of rows a request, with and without a past, beside a decoding request and one with nothing."""
+    st = _attention_state(NKV, ratio, hs, bs, [700, 512, 130, 0, 333], [512, 512, 101, 0, 1], 76)
+    _check_attention(st, _attend(st, 512))
